@@ -84,7 +84,7 @@ extern "C" {
 
 /* Bumped whenever an entry point is added or changes its signature, or a workspace its layout; a binding compares it
  * with the header it was written against. */
-#define VAMD_ABI_VERSION 7
+#define VAMD_ABI_VERSION 8
 int vamd_abi_version(void);
 const char* vamd_last_error(void);
 
@@ -245,6 +245,39 @@ int vamd_row_softmax_backward_as(const void* logits, int dtype, int64_t n_rows, 
 int vamd_row_softmax_backward_add(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t ld,
                                   const int64_t* labels, const float* lse, const float* mean_z, const void* d_logprobs,
                                   const void* d_entropy, int grad_dtype, void* d_logits, int64_t ld_out, void* stream);
+/* Top alternatives of a row beside the log-prob of a given token and the entropy, of softmax(logits / temperature):
+ *   top [n_rows, k] fp32 and index [n_rows, k]: the log-probs of the k largest logits, largest first, the lowest index first
+ *   among equals (a NaN ranks below -inf), 1 <= k <= min(VAMD_TOPK_MAX, vocab);
+ *   logprobs (needs labels; a label outside [0, vocab) yields 0) and entropy (a logit of -inf adds nothing): fp32 [n_rows], may
+ *   be NULL; stats: fp32 [n_rows, 4], 16-byte aligned, for the backward pass, may be NULL.
+ * One pass over the logits.  Few rows are shared out over workgroups and need a workspace (0 bytes otherwise). */
+#define VAMD_TOPK_MAX 256
+size_t vamd_row_topk_workspace_bytes(int64_t n_rows, int64_t vocab, int dtype, int k);
+int vamd_row_topk(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t ld, const int64_t* labels, int k,
+                  float rcp_temperature, float* logprobs, float* entropy, float* top, int64_t* index, float* stats,
+                  void* workspace, size_t workspace_bytes, void* stream);
+/* Its gradient for upstream gradients of logprobs, entropy [n_rows] and top [n_rows, k], fp32, each of which may be NULL;
+ * row_scratch: fp32 [n_rows].  d_logits has the element type of the logits, row pitch ld_out, and is another buffer. */
+int vamd_row_topk_backward(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t ld, const int64_t* labels,
+                           int k, const int64_t* index, float rcp_temperature, const float* stats, const float* d_logprobs,
+                           const float* d_entropy, const float* d_top, float* row_scratch, void* d_logits, int64_t ld_out,
+                           void* stream);
+/* Divergence of q = softmax(logits / temperature) from a teacher's k tokens (teacher_index, int64) with log-probs t
+ * (teacher_logprobs, fp32), both [n_rows, k], p = exp(t), per row:
+ *   VAMD_DIV_FORWARD_KL sum p (t - log q), VAMD_DIV_REVERSE_KL sum q (log q - t), VAMD_DIV_JSD beta sum p (t - log w) +
+ *   (1 - beta) sum q (log q - log w) with w = beta p + (1 - beta) q, 0 < beta < 1.
+ * An entry whose index lies outside [0, vocab) or whose t is -inf adds nothing; a row of such entries has loss 0 and no gradient.
+ * stats (fp32 [n_rows, 4], 16-byte aligned) and slope (fp32 [n_rows, k], d loss / d log q) are what the backward pass needs, and
+ * may be NULL without one. */
+#define VAMD_DIV_FORWARD_KL 0
+#define VAMD_DIV_REVERSE_KL 1
+#define VAMD_DIV_JSD 2
+int vamd_row_divergence(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t ld,
+                        const float* teacher_logprobs, const int64_t* teacher_index, int k, int divergence, float beta,
+                        float rcp_temperature, float* loss, float* stats, float* slope, void* stream);
+int vamd_row_divergence_backward(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t ld,
+                                 const int64_t* teacher_index, int k, float rcp_temperature, const float* stats,
+                                 const float* slope, const float* d_loss, void* d_logits, int64_t ld_out, void* stream);
 /* clip_by_value (verl/utils/torch_functional.py:203-221): out = max(min(x, hi), lo) over n fp32 elements, and its
  * gradients with torch's rule for binary min / max (the selected operand takes the gradient, equal operands half
  * each); d_x / d_lo / d_hi may be NULL.  A NaN in x, lo or hi gives a NaN output, as torch.min / torch.max of two

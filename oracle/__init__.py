@@ -12,8 +12,9 @@ fallback and raises when the HIP library is missing.
 Parity status: every function here is pinned by ``tests/test_oracle_*.py``
 against the reference-held vectors (masked_mean cases, group_mean_std known
 answer, GAE multi-turn fixture, GRPO loop==vectorised grids), against
-closed forms, fp64 brute-force scalar loops and torch.autograd.  No function is
-"parity unpinned".
+closed forms, fp64 brute-force scalar loops and torch.autograd.  The functions
+of ``topk.py`` have no counterpart there ("parity unpinned"): they are checked
+against hand-computed values.
 """
 
 from .head import (  # noqa: F401
@@ -33,6 +34,10 @@ from .masked import (  # noqa: F401
     masked_var,
     masked_whiten,
     sum_pi_squared_from_logits,
+)
+from .topk import (  # noqa: F401
+    topk_distillation,
+    topk_logprobs,
 )
 from .advantages import (  # noqa: F401
     gae_advantage_return,

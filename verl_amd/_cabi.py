@@ -70,6 +70,15 @@ SIGNATURES = {
                                              c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p]),
     "vamd_row_softmax_backward_add": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
                                              c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p]),
+    "vamd_row_topk_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int, c_int]),
+    "vamd_row_topk": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int, c_float, c_void_p, c_void_p,
+                              c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "vamd_row_topk_backward": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int, c_void_p, c_float,
+                                       c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "vamd_row_divergence": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int, c_float,
+                                    c_float, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "vamd_row_divergence_backward": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int, c_float, c_void_p,
+                                             c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     "vamd_clip_by_value": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
     "vamd_clip_by_value_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
                                             c_void_p, c_void_p]),
@@ -154,7 +163,7 @@ def lib_path() -> str:
     return _LIB_PATH
 
 
-ABI_VERSION = 7  # VAMD_ABI_VERSION of include/verl_amd.h
+ABI_VERSION = 8  # VAMD_ABI_VERSION of include/verl_amd.h
 
 
 def load_library(path: str | None = None) -> ctypes.CDLL:

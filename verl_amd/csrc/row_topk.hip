@@ -1,0 +1,862 @@
+// The k largest logits of a row as log-probabilities, beside the log-probability of a given token and the entropy; and the
+// divergence of a row's softmax from a teacher's k most likely tokens.  Both with their gradients.
+//
+// With y = z log2(e) / T, m = max y and s = sum 2^(y - m):  log q_j = ((y_j - m) - log2 s) ln 2.
+//   top alternatives: the k largest z, the lowest column first among equals (-0 equals 0; a NaN is below everything, and every
+//     log-probability of its row is NaN); entropy = lse - sum q z / T, where q = 0 adds nothing, so that logits of -inf are allowed
+//   divergence, over a teacher's tokens i_k with log-probabilities t_k, p = exp(t_k), q = q at i_k, b = beta:
+//     forward KL  sum p (t - log q)                                  c_k = -p
+//     reverse KL  sum q (log q - t)                                  c_k = q (log q - t + 1)
+//     JSD         b sum p (t - log w) + (1 - b) sum q (log q - log w)   c_k = (1 - b) q (log q - log w),  w = b p + (1 - b) q
+//     where c_k = d loss / d log q_k, and an entry outside [0, vocab), or whose t is -inf, adds nothing
+//   gradients: d z_j = (sum_k g_k [j = i_k] - q_j sum_k g_k) / T for upstream gradients g_k of log q at i_k, and for the entropy
+//     -g q_j (z_j - mean) / T^2
+// Bound by HBM: the logits are read once, backward read and written once.
+#include "common.h"
+#include "logit_rows.h"
+
+namespace vamd {
+namespace {
+
+constexpr int kNarrow = 256, kWide = 1024;  // threads per workgroup
+constexpr int kMaxK = VAMD_TOPK_MAX;
+constexpr float kInf = __builtin_huge_valf();
+
+struct Softmax {
+  float m, s, sz;  // max y, sum 2^(y - m), sum 2^(y - m) z
+};
+__device__ __forceinline__ void merge(Softmax& a, const Softmax& b) {
+  const float m = fmaxf(a.m, b.m);
+  const float x = __builtin_amdgcn_exp2f(a.m - m), y = __builtin_amdgcn_exp2f(b.m - m);
+  a = Softmax{m, a.s * x + b.s * y, a.sz * x + b.sz * y};
+}
+// log q of logit z; the lowest values of a type, which masks are made of, would overflow as y
+__device__ __forceinline__ float log_q(float z, float scale2, const Softmax& r) {
+  const float log2_s = log2f(r.s);
+  return z < -1.0e30f ? fmaf(z, scale2 * kLn2, -(r.m + log2_s) * kLn2) : (fmaf(z, scale2, -r.m) - log2_s) * kLn2;
+}
+
+// One thread's part of the columns [begin, end).  TOP: beside the softmax state the largest logit of each of the thread's groups,
+// a group being `span` trips of kInFlight 16-byte loads, goes to LDS; `best` is the largest of all.  SUM_Z: whether sz is wanted.
+template <class D, bool VEC, bool STREAM, int NT, bool TOP, bool SUM_Z>
+__device__ __forceinline__ void walk(const typename D::type* __restrict__ row, int64_t begin, int64_t end, float scale2,
+                                     int span, Softmax& st, float& best, float* groups) {
+  constexpr int G = D::kVec;
+  constexpr int64_t stride = (int64_t)NT * G;
+  float m = kNegBig, s = 0.f, sz = 0.f, held = -kInf;
+  int left = span, slot = threadIdx.x;
+  best = -kInf;
+  for (int64_t base = begin; base < end; base += stride * kInFlight) {  // the same trips for every thread
+    const int64_t c0 = base + (int64_t)threadIdx.x * G;
+    u32x4_t raw[kInFlight];
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      const int64_t c = c0 + u * stride;
+      if (c + G <= end) raw[u] = load_whole<D, VEC, STREAM>(row + c);
+    }
+    float x[kInFlight][G];
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      const int64_t c = c0 + u * stride;
+      if (c + G <= end) {
+        const Pack<D> p = __builtin_bit_cast(Pack<D>, raw[u]);
+#pragma unroll
+        for (int e = 0; e < G; ++e) x[u][e] = to_float(p.v[e], D());
+      } else {
+        load_ragged<D>(row, c, end, -kInf, x[u]);
+      }
+    }
+    float hi = -kInf, lo = kInf;
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u)
+#pragma unroll
+      for (int e = 0; e < G; ++e) {
+        hi = fmaxf(hi, x[u][e]);
+        if (SUM_Z) lo = fminf(lo, x[u][e]);
+      }
+    if constexpr (TOP) {
+      held = fmaxf(held, hi);
+      if (--left == 0 || base + stride * kInFlight >= end) {
+        groups[slot] = held;
+        best = fmaxf(best, held);
+        held = -kInf;
+        slot += NT;
+        left = span;
+      }
+    }
+    const float y = hi * scale2;
+    if (y > m) {
+      const float resc = __builtin_amdgcn_exp2f(m - y);
+      s *= resc;
+      sz *= resc;
+      m = y;
+    }
+    if (SUM_Z && __builtin_expect(lo == -kInf, 0)) {  // masked logits, or none: 2^(-inf) (-inf) is 0 here and not NaN
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u)
+#pragma unroll
+        for (int e = 0; e < G; ++e) {
+          const float z = x[u][e];
+          const float ex = z == -kInf ? 0.f : __builtin_amdgcn_exp2f(fmaf(z, scale2, -m));
+          s += ex;
+          sz = fmaf(ex, z == -kInf ? 0.f : z, sz);
+        }
+    } else {
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u)
+#pragma unroll
+        for (int e = 0; e < G; ++e) {
+          const float z = x[u][e];
+          const float ex = __builtin_amdgcn_exp2f(fmaf(z, scale2, -m));
+          s += ex;
+          if (SUM_Z) sz = fmaf(ex, z, sz);
+        }
+    }
+  }
+  st = Softmax{m, s, sz};
+}
+
+// the wavefront's state in every lane
+__device__ __forceinline__ void merge_wave(Softmax& st) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1)
+    merge(st, Softmax{__shfl_xor(st.m, off, 64), __shfl_xor(st.s, off, 64), __shfl_xor(st.sz, off, 64)});
+}
+
+// ---- the k largest of a range of a row ------------------------------------------------------------------------
+// A logit as a number that orders like it, -0 as 0, NaN lowest; with its column below it, so that the largest comes first and
+// among equals the lowest column, and no two are the same.
+__device__ __forceinline__ unsigned order_of(float z) {
+  const unsigned b = __float_as_uint(z + 0.f);
+  return z != z ? 0u : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+constexpr unsigned kOrderOfMinusInf = 0x007fffffu;
+__device__ __forceinline__ float logit_of(unsigned order) {
+  return order == 0u ? __builtin_nanf("") : __uint_as_float((order & 0x80000000u) ? order & 0x7fffffffu : ~order);
+}
+__device__ __forceinline__ uint64_t entry_of(unsigned order, int64_t col) {
+  return (uint64_t)order << 32 | (0xffffffffu - (unsigned)col);
+}
+__device__ __forceinline__ unsigned order_in(uint64_t entry) { return (unsigned)(entry >> 32); }
+__device__ __forceinline__ int64_t column_in(uint64_t entry) { return (int64_t)(0xffffffffu - (unsigned)entry); }
+
+// The walk leaves the maximum of every group in LDS (at most kGroupBytes of them; a row of 152064 bf16 has 4864 groups of 32
+// logits).  The k-th largest of the threads' own maxima is a value that at least k logits reach; only groups that reach it can hold
+// one of the k largest, and these, about k of them, are read again from the caches: k x 64 bytes instead of the row.  What reaches
+// the value there, a little more than k logits, is ranked by counting.  Where that list would be too long (many equal logits)
+// the order of the k-th largest is found digit by digit in passes over the row, which is right for any values.
+constexpr int kGroupBytes = 20 * 1024, kGroupList = 512, kCandidates = 1024;
+
+template <int NT>
+struct PickLds {
+  unsigned top[NT];  // the threads' maxima; later the digit counts
+  int group[kGroupList];
+  float red[3][NT / 64];
+  Softmax whole;
+  unsigned least;
+  int groups, candidates, digit, above, wave[NT / 64];
+};
+
+// the state of the whole workgroup, and for pick() the value that at least k logits reach, in `least`
+template <class D, int NT>
+__device__ __forceinline__ void meet(PickLds<NT>& lds, Softmax st, float best, int k) {
+  // bits below it cannot tell two logits of the type apart (fp32: change the value by less than 2^-14)
+  constexpr int kLowBit = std::is_same_v<D, BF16> ? 16 : std::is_same_v<D, F16> ? 13 : 9;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  merge_wave(st);
+  if (lane == 0) {
+    lds.red[0][w] = st.m;
+    lds.red[1][w] = st.s;
+    lds.red[2][w] = st.sz;
+  }
+  lds.top[threadIdx.x] = order_of(best);
+  if (threadIdx.x == 0) lds.groups = lds.candidates = 0;
+  __syncthreads();
+  if (w == 1) {
+    Softmax all{lds.red[0][0], lds.red[1][0], lds.red[2][0]};
+#pragma unroll
+    for (int j = 1; j < NT / 64; ++j) merge(all, Softmax{lds.red[0][j], lds.red[1][j], lds.red[2][j]});
+    if (lane == 0) lds.whole = all;
+  } else if (w == 0) {
+    constexpr int P = NT / 64;
+    unsigned mine[P];
+#pragma unroll
+    for (int j = 0; j < P; ++j) mine[j] = lds.top[j * 64 + lane];
+    const auto reach = [&](unsigned order) {
+      int n = 0;
+#pragma unroll
+      for (int j = 0; j < P; ++j) n += __popcll(__ballot(mine[j] >= order));
+      return n;
+    };
+    unsigned least = kOrderOfMinusInf + 1;  // fewer than k threads with a finite logit: every finite one
+    if (reach(least) >= k) {
+      unsigned order = 0;
+      for (int bit = 31; bit >= kLowBit; --bit)
+        if (reach(order | 1u << bit) >= k) order |= 1u << bit;
+      if (order > least) least = order;
+    }
+    if (lane == 0) lds.least = least;
+  }
+  __syncthreads();
+}
+
+// emit(rank, entry) for each entry of the list that is among its k largest
+template <int NT, class Emit>
+__device__ __forceinline__ void rank_list(const uint64_t* list, int n, int k, Emit&& emit) {
+  for (int j = threadIdx.x; j < n; j += NT) {
+    const uint64_t mine = list[j];
+    int rank = 0;
+    for (int i = 0; i < n; ++i) rank += list[i] > mine;
+    if (rank < k) emit(rank, mine);
+  }
+}
+
+// emit(rank, entry) for the first `need` columns of the range whose logit is of this order, from `rank` on; returns how many
+template <class D, int NT, class Emit>
+__device__ int rank_equal(PickLds<NT>& lds, const typename D::type* __restrict__ row, int64_t begin, int64_t end,
+                          unsigned order, int need, int rank, Emit&& emit) {
+  constexpr int G = D::kVec;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int found = 0;
+  for (int64_t base = begin; base < end && found < need; base += (int64_t)NT * G) {
+    const int64_t c = base + (int64_t)threadIdx.x * G;
+    unsigned here = 0;
+#pragma unroll
+    for (int e = 0; e < G; ++e)
+      if (c + e < end && order_of(to_float(row[c + e], D())) == order) here |= 1u << e;
+    const int n = __popc(here);
+    int before = n;  // in this and lower lanes
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int x = __shfl_up(before, off, 64);
+      if (lane >= off) before += x;
+    }
+    __syncthreads();
+    if (lane == 63) lds.wave[w] = before;
+    __syncthreads();
+    int place = found + before - n, all = found;
+    for (int j = 0; j < NT / 64; ++j) {
+      if (j < w) place += lds.wave[j];
+      all += lds.wave[j];
+    }
+#pragma unroll
+    for (int e = 0; e < G; ++e)
+      if (here >> e & 1u) {
+        if (place < need) emit(rank + place, entry_of(order, c + e));
+        ++place;
+      }
+    found = all;
+  }
+  return found < need ? found : need;
+}
+
+// by digits: passes over the range, for any values
+template <class D, int NT, class Emit>
+__device__ void pick_by_digits(PickLds<NT>& lds, uint64_t* list, const typename D::type* __restrict__ row, int64_t begin,
+                               int64_t end, int k, Emit&& emit) {
+  const int kk = (int)(end - begin < k ? end - begin : k);
+  unsigned order = 0, known = 0;
+  int need = kk;
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    __syncthreads();
+    for (int j = threadIdx.x; j < 256; j += NT) lds.top[j] = 0;
+    __syncthreads();
+    for (int64_t c = begin + threadIdx.x; c < end; c += NT) {
+      const unsigned o = order_of(to_float(row[c], D()));
+      if ((o & known) != order) continue;
+      const unsigned digit = o >> shift & 255u;
+      // one addition for a wavefront of equal digits
+      const uint64_t active = __ballot(true);
+      if (__ballot(digit == (unsigned)__builtin_amdgcn_readfirstlane((int)digit)) == active) {
+        if ((int)(threadIdx.x & 63) == __ffsll((unsigned long long)active) - 1) atomicAdd(&lds.top[digit], (unsigned)__popcll(active));
+      } else {
+        atomicAdd(&lds.top[digit], 1u);
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      int above = 0, digit = 255;
+      while (digit > 0 && above + (int)lds.top[digit] < need) above += (int)lds.top[digit--];
+      lds.digit = digit;
+      lds.above = above;
+    }
+    __syncthreads();
+    order |= (unsigned)lds.digit << shift;
+    known |= 255u << shift;
+    need -= lds.above;
+  }
+  // kk - need logits are above the k-th largest, `need` of its equals belong to the k
+  if (threadIdx.x == 0) lds.candidates = 0;
+  __syncthreads();
+  for (int64_t c = begin + threadIdx.x; c < end; c += NT) {
+    const unsigned o = order_of(to_float(row[c], D()));
+    if (o > order) list[atomicAdd(&lds.candidates, 1)] = entry_of(o, c);
+  }
+  __syncthreads();
+  rank_list<NT>(list, kk - need, k, emit);
+  rank_equal<D, NT>(lds, row, begin, end, order, need, kk - need, emit);
+}
+
+// emit(rank, entry) once for every rank below k that the range has, by any thread.  `groups`: the maxima that the walk left in
+// LDS, at least kCandidates entries long; they are overwritten.  meet() has run.
+template <class D, bool VEC, int NT, class Emit>
+__device__ __forceinline__ void pick(PickLds<NT>& lds, float* groups, const typename D::type* __restrict__ row, int64_t begin,
+                                     int64_t end, int span, int k, float best, Emit&& emit) {
+  constexpr int G = D::kVec;
+  const int64_t trip = (int64_t)NT * G * kInFlight;
+  const int trips = (int)((end - begin + trip - 1) / trip), slots = (trips + span - 1) / span * NT;
+  const float least = logit_of(lds.least);
+  const bool all_finite = lds.least == kOrderOfMinusInf + 1;
+  if (best >= least)
+    for (int slot = threadIdx.x; slot < slots; slot += NT)
+      if (groups[slot] >= least) {
+        const int at = atomicAdd(&lds.groups, 1);
+        if (at < kGroupList) lds.group[at] = slot;
+      }
+  __syncthreads();
+  uint64_t* const list = reinterpret_cast<uint64_t*>(groups);
+  const int pieces = kInFlight * span, n_groups = lds.groups;
+  if (n_groups <= kGroupList) {
+    for (int j = threadIdx.x; j < n_groups * pieces; j += NT) {
+      const int slot = lds.group[j / pieces];
+      const int64_t c = begin + ((int64_t)(slot / NT * pieces + j % pieces) * NT + slot % NT) * G;
+      float x[G];
+      if (c + G <= end) {
+        const Pack<D> p = __builtin_bit_cast(Pack<D>, load_whole<D, VEC, false>(row + c));
+#pragma unroll
+        for (int e = 0; e < G; ++e) x[e] = to_float(p.v[e], D());
+      } else {
+        load_ragged<D>(row, c, end, -kInf, x);
+      }
+#pragma unroll
+      for (int e = 0; e < G; ++e)
+        if (x[e] >= least) {
+          const int at = atomicAdd(&lds.candidates, 1);
+          if (at < kCandidates) list[at] = entry_of(order_of(x[e]), c + e);
+        }
+    }
+    __syncthreads();
+    const int n = lds.candidates;
+    if (n <= kCandidates) {
+      rank_list<NT>(list, n, k, emit);
+      if (n < k && all_finite) {
+        // the others are -inf, and then NaN, in the order of their columns
+        const int64_t more = end - begin - n;
+        const int need = (int)(more < k - n ? more : k - n);
+        const int got = rank_equal<D, NT>(lds, row, begin, end, kOrderOfMinusInf, need, n, emit);
+        rank_equal<D, NT>(lds, row, begin, end, 0u, need - got, n + got, emit);
+      }
+      return;
+    }
+  }
+  pick_by_digits<D, NT>(lds, list, row, begin, end, k, emit);
+}
+
+struct TopkArgs {
+  const void* logits;
+  int64_t ld, cols;
+  const int64_t* labels;
+  int k, span;
+  float scale2, rcp_t;
+  float* logprobs;
+  float* entropy;
+  float* top;      // [rows][k]
+  int64_t* index;  // [rows][k]
+  float4* stats;   // m, 1 / s, mean z, lse
+  int64_t cached_rows;
+  int splits;  // of a row; more than one: each leaves its state and its k largest, for row_topk_join_kernel
+  int64_t split_cols;
+  float4* part_state;     // [rows][splits]
+  uint64_t* part_entry;  // [rows][splits][k], largest first, 0 where there are fewer
+};
+
+struct RowResult {
+  const TopkArgs& a;
+  int64_t r;
+  Softmax st;
+  __device__ __forceinline__ void operator()(int rank, uint64_t entry) const {
+    a.top[r * a.k + rank] = log_q(logit_of(order_in(entry)), a.scale2, st);
+    a.index[r * a.k + rank] = column_in(entry);
+  }
+  template <class D>
+  __device__ __forceinline__ void scalars(const typename D::type* __restrict__ row) const {
+    const float lse = (st.m + log2f(st.s)) * kLn2, mean = st.sz / st.s;
+    if (a.entropy) a.entropy[r] = fmaf(-mean, a.rcp_t, lse);
+    if (a.stats) a.stats[r] = make_float4(st.m, 1.f / st.s, mean, lse);
+    if (a.logprobs) {  // a label outside [0, cols) reads nothing and yields 0
+      const int64_t label = a.labels[r];
+      a.logprobs[r] = label >= 0 && label < a.cols ? log_q(to_float(row[label], D()), a.scale2, st) : 0.f;
+    }
+  }
+};
+
+template <class D, bool VEC, int NT>
+__global__ __launch_bounds__(NT) void row_topk_kernel(TopkArgs a) {
+  using T = typename D::type;
+  extern __shared__ __attribute__((aligned(16))) float groups[];
+  __shared__ PickLds<NT> lds;
+  const int64_t r = a.splits > 1 ? blockIdx.x / a.splits : blockIdx.x;
+  const int split = a.splits > 1 ? (int)(blockIdx.x % a.splits) : 0;
+  const int64_t begin = split * a.split_cols, end = begin + a.split_cols < a.cols ? begin + a.split_cols : a.cols;
+  const T* __restrict__ row = static_cast<const T*>(a.logits) + r * a.ld;
+  Softmax st;
+  float best;
+  if (r < a.cached_rows) walk<D, VEC, false, NT, true, true>(row, begin, end, a.scale2, a.span, st, best, groups);
+  else walk<D, VEC, true, NT, true, true>(row, begin, end, a.scale2, a.span, st, best, groups);
+  meet<D, NT>(lds, st, best, a.k);
+  st = lds.whole;
+  if (a.splits > 1) {
+    const int64_t part = r * a.splits + split;
+    uint64_t* const out = a.part_entry + part * a.k;
+    pick<D, VEC, NT>(lds, groups, row, begin, end, a.span, a.k, best, [&](int rank, uint64_t entry) { out[rank] = entry; });
+    for (int64_t j = end - begin + threadIdx.x; j < a.k; j += NT) out[j] = 0;
+    if (threadIdx.x == 0) a.part_state[part] = make_float4(st.m, st.s, st.sz, 0.f);
+  } else {
+    const RowResult result{a, r, st};
+    pick<D, VEC, NT>(lds, groups, row, begin, end, a.span, a.k, best, result);
+    if (threadIdx.x == 0) result.template scalars<D>(row);
+  }
+}
+
+// A row's splits: an entry's rank is its place in its own list plus how many of the other lists' are larger.
+template <class D>
+__global__ __launch_bounds__(kNarrow) void row_topk_join_kernel(TopkArgs a) {
+  extern __shared__ __attribute__((aligned(16))) float groups[];
+  uint64_t* const list = reinterpret_cast<uint64_t*>(groups);
+  __shared__ Softmax whole;
+  const int64_t r = blockIdx.x;
+  const int n = a.splits * a.k;
+  for (int j = threadIdx.x; j < n; j += kNarrow) list[j] = a.part_entry[r * n + j];
+  if (threadIdx.x < 64) {
+    Softmax st{kNegBig, 0.f, 0.f};
+    for (int j = threadIdx.x; j < a.splits; j += 64) {
+      const float4 x = a.part_state[r * a.splits + j];
+      merge(st, Softmax{x.x, x.y, x.z});
+    }
+    merge_wave(st);
+    if (threadIdx.x == 0) whole = st;
+  }
+  __syncthreads();
+  const RowResult result{a, r, whole};
+  for (int j = threadIdx.x; j < n; j += kNarrow) {
+    const uint64_t mine = list[j];
+    if (mine == 0) continue;
+    const int own = j / a.k;
+    int rank = j - own * a.k;
+    for (int other = 0; other < a.splits && rank < a.k; ++other) {
+      if (other == own) continue;
+      int lo = 0, hi = a.k;  // how many of a list that falls are larger
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (list[other * a.k + mid] > mine) lo = mid + 1;
+        else hi = mid;
+      }
+      rank += lo;
+    }
+    if (rank < a.k) result(rank, mine);
+  }
+  if (threadIdx.x == 0) result.template scalars<D>(static_cast<const typename D::type*>(a.logits) + r * a.ld);
+}
+
+// ---- divergence from a teacher's tokens -----------------------------------------------------------------------
+struct Term {
+  float loss, slope;  // of a teacher's token, and its derivative with respect to log q
+};
+// Differences of logarithms are formed from d = log q - t, so that nothing cancels where the two agree.
+__device__ __forceinline__ Term divergence_term(int kind, float beta, float t, float lq) {
+  const float p = expf(t), q = expf(lq), d = lq - t;
+  if (kind == VAMD_DIV_FORWARD_KL) return Term{p > 0.f ? -p * d : 0.f, -p};
+  if (kind == VAMD_DIV_REVERSE_KL) {
+    const float x = q == 0.f ? 0.f : q * d;
+    return Term{x, x + q};
+  }
+  // t - log w and log q - log w
+  float a, b;
+  if (d > 0.f) {
+    b = -log1pf(beta * expm1f(-d));
+    a = b - d;
+  } else {
+    a = -log1pf((1.f - beta) * expm1f(d));
+    b = d + a;
+  }
+  const float x = q == 0.f ? 0.f : (1.f - beta) * q * b;
+  return Term{(p == 0.f ? 0.f : beta * p * a) + x, x};
+}
+
+struct DivergenceArgs {
+  const void* logits;
+  int64_t ld, cols;
+  const float* teacher;  // [rows][k] log-probabilities
+  const int64_t* index;  // [rows][k]
+  int k, kind;
+  float beta, scale2;
+  float* loss;
+  float4* stats;  // m, 1 / s, sum of the slopes, lse
+  float* slope;   // [rows][k]
+  int64_t cached_rows;
+};
+
+template <class D, bool VEC, int NT>
+__global__ __launch_bounds__(NT) void row_divergence_kernel(DivergenceArgs a) {
+  using T = typename D::type;
+  __shared__ float red[2][NT / 64];
+  const int64_t r = blockIdx.x;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const T* __restrict__ row = static_cast<const T*>(a.logits) + r * a.ld;
+  // requested before the walk: they are a chain of two trips behind it otherwise
+  int64_t index = -1;
+  float t = -kInf, z = 0.f;
+  if ((int)threadIdx.x < a.k) {
+    index = a.index[r * a.k + threadIdx.x];
+    t = a.teacher[r * a.k + threadIdx.x];
+    if (index >= 0 && index < a.cols && t != -kInf) z = to_float(row[index], D());
+    else index = -1;
+  }
+  Softmax st;
+  float best;
+  if (r < a.cached_rows) walk<D, VEC, false, NT, false, false>(row, 0, a.cols, a.scale2, 1, st, best, nullptr);
+  else walk<D, VEC, true, NT, false, false>(row, 0, a.cols, a.scale2, 1, st, best, nullptr);
+  merge_wave(st);
+  if (lane == 0) {
+    red[0][w] = st.m;
+    red[1][w] = st.s;
+  }
+  __syncthreads();
+  st = Softmax{red[0][0], red[1][0], 0.f};
+#pragma unroll
+  for (int j = 1; j < NT / 64; ++j) merge(st, Softmax{red[0][j], red[1][j], 0.f});
+  Term mine{0.f, 0.f};
+  if (index >= 0) mine = divergence_term(a.kind, a.beta, t, log_q(z, a.scale2, st));
+  if (a.slope && (int)threadIdx.x < a.k) a.slope[r * a.k + threadIdx.x] = mine.slope;
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    mine.loss += __shfl_xor(mine.loss, off, 64);
+    mine.slope += __shfl_xor(mine.slope, off, 64);
+  }
+  __syncthreads();
+  if (lane == 0) {
+    red[0][w] = mine.loss;
+    red[1][w] = mine.slope;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    constexpr int W = kMaxK / 64;  // the wavefronts that hold entries
+    float loss = 0.f, slope = 0.f;
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      loss += red[0][j];
+      slope += red[1][j];
+    }
+    a.loss[r] = loss;
+    if (a.stats) a.stats[r] = make_float4(st.m, 1.f / st.s, slope, (st.m + log2f(st.s)) * kLn2);
+  }
+}
+static_assert(kMaxK <= kNarrow, "an entry per thread");
+
+// ---- gradient --------------------------------------------------------------------------------------------------
+// d z_j = sum_k scale g_k [j = i_k] / T + g_lp [j = label] / T - q_j (scale weight / T + g_ent (z_j - mean z) / T^2)
+struct EntriesArgs {
+  const void* logits;
+  int64_t ld, cols;
+  int chunks, k;
+  const int64_t* index;    // [rows][k]; one outside [0, cols) matches nothing
+  const float* grad;       // [rows][k]: g_k
+  const float4* stats;     // m, 1 / s, ., .
+  const float* weight;     // [rows]: sum of all g; null: the third of stats
+  const float* scale;      // [rows] or null (1)
+  const int64_t* labels;   // with d_logprobs
+  const float* d_logprobs;
+  const float* d_entropy;  // with it the third of stats is the mean of z
+  float scale2, rcp_t;
+  void* out;
+  int64_t ld_out;
+};
+
+// One workgroup per (row, chunk of kNarrow * G * F columns), as row_softmax_backward_kernel, whose comments say why.  Every
+// wavefront looks through the row's entries for those of its own columns, 64 at a time, and adds them, in their order, in the
+// registers of the lane that holds the column: an index that comes twice counts twice, and each gradient is rounded once.
+template <class D, bool VEC, bool STREAM>
+__global__ __launch_bounds__(kNarrow) void row_entries_backward_kernel(EntriesArgs a) {
+  using T = typename D::type;
+  constexpr int G = D::kVec, F = D::kBackwardLoads;
+  const int64_t r = blockIdx.x / a.chunks;
+  const int chunk = blockIdx.x % a.chunks, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const T* __restrict__ row = static_cast<const T*>(a.logits) + r * a.ld;
+  T* __restrict__ out = static_cast<T*>(a.out) + r * a.ld_out;
+  constexpr int64_t stride = (int64_t)kNarrow * G;
+  const int64_t first = (int64_t)chunk * stride * F, c0 = first + (int64_t)threadIdx.x * G;
+  u32x4_t raw[F];
+#pragma unroll
+  for (int u = 0; u < F; ++u) {
+    const int64_t c = c0 + u * stride;
+    if (c + G <= a.cols) raw[u] = load_whole<D, VEC, STREAM>(row + c);
+  }
+  const int64_t* const entries = a.index + r * a.k;
+  int64_t entry = lane < a.k ? entries[lane] : -1;
+  __builtin_amdgcn_sched_barrier(0);
+  const float4 st = a.stats[r];
+  const float scale = (a.scale ? a.scale[r] : 1.f) * a.rcp_t;
+  const float glp = a.d_logprobs ? a.d_logprobs[r] * a.rcp_t : 0.f;
+  const int64_t label = a.d_logprobs ? a.labels[r] : -1;
+  const float u0 = scale * (a.weight ? a.weight[r] : st.z) * st.y;
+  const float u1 = a.d_entropy ? a.d_entropy[r] * a.rcp_t * a.rcp_t * st.y : 0.f;
+  float x[F][G];
+#pragma unroll
+  for (int u = 0; u < F; ++u) {
+    const int64_t c = c0 + u * stride;
+    if (c + G <= a.cols) {
+      const Pack<D> p = __builtin_bit_cast(Pack<D>, raw[u]);
+#pragma unroll
+      for (int e = 0; e < G; ++e) x[u][e] = to_float(p.v[e], D());
+    } else {
+      load_ragged<D>(row, c, a.cols, 0.f, x[u]);
+    }
+    const int64_t hit64 = label - c;
+    const int hit = (hit64 >= 0 && hit64 < G) ? (int)hit64 : -1;
+#pragma unroll
+    for (int e = 0; e < G; ++e) {
+      const float z = x[u][e];
+      const float ex = __builtin_amdgcn_exp2f(fmaf(z, a.scale2, -st.x));
+      const float t = fmaf(u1, fmaxf(z, -1.0e20f) - st.z, u0);  // below it q is 0, which -inf would make a NaN
+      x[u][e] = fmaf(-ex, a.d_entropy ? t : u0, hit == e ? glp : 0.f);
+    }
+  }
+  for (int e0 = 0; e0 < a.k; e0 += 64) {
+    if (e0 > 0) entry = e0 + lane < a.k ? entries[e0 + lane] : -1;
+    const int64_t rel64 = entry - first;
+    const bool inside = entry < a.cols && rel64 >= 0 && rel64 < stride * F;
+    const int rel = inside ? (int)rel64 : 0;
+    uint64_t hits = __ballot(inside && rel / G % kNarrow / 64 == w);
+    while (hits) {
+      const int b = __ffsll((unsigned long long)hits) - 1;
+      hits &= hits - 1;
+      const int at = __builtin_amdgcn_readlane(rel, b);
+      const float g = a.grad[r * a.k + e0 + b] * scale;
+      const int mine = at / G % 64 == lane ? at / (int)stride * G + at % G : -1;
+#pragma unroll
+      for (int u = 0; u < F; ++u)
+#pragma unroll
+        for (int e = 0; e < G; ++e) x[u][e] += mine == u * G + e ? g : 0.f;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < F; ++u) {
+    const int64_t c = c0 + u * stride;
+    if (c < a.cols) store_group<D, VEC>(out, c, a.cols, x[u]);
+  }
+}
+
+// weight[r] = d_logprobs[r], where the label counts, + sum of d_top[r]; a wavefront per row
+__global__ __launch_bounds__(kNarrow) void row_topk_weight_kernel(const float* d_logprobs, const int64_t* labels, int64_t cols,
+                                                                  const float* d_top, int k, int64_t rows, float* weight) {
+  const int64_t r = (int64_t)blockIdx.x * (kNarrow / 64) + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (r >= rows) return;
+  float sum = 0.f;
+  for (int j = lane; j < k; j += 64) sum += d_top[r * k + j];
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+  if (lane != 0) return;
+  if (d_logprobs && labels[r] >= 0 && labels[r] < cols) sum += d_logprobs[r];
+  weight[r] = sum;
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------
+// Up to 64 alternatives the maxima of 256 threads give a value that about k logits reach; for more, 1024 threads.
+int threads_for(int k) { return k <= 64 ? kNarrow : kWide; }
+
+constexpr int kJoinEntries = 6144;  // 48 KB of LDS in row_topk_join_kernel
+
+struct TopkPlan {
+  int threads, span, splits;
+  int64_t split_cols, slots;  // slots: group maxima per workgroup
+  size_t lds_bytes() const {
+    const size_t list = kCandidates * sizeof(uint64_t), maxima = (size_t)slots * sizeof(float);
+    return maxima > list ? maxima : list;
+  }
+};
+TopkPlan plan_topk(int64_t n_rows, int64_t vocab, int dtype, int k) {
+  TopkPlan p;
+  p.threads = threads_for(k);
+  const int64_t trip = (int64_t)p.threads * (dtype == VAMD_DT_F32 ? 4 : 8) * kInFlight;
+  int64_t trips = (vocab + trip - 1) / trip;
+  // Few rows: a row is shared out over workgroups, a trip or more each, until there are four to a CU.
+  const int64_t workgroups = (int64_t)device_cu_count() * (4 * kNarrow / p.threads);
+  int64_t splits = n_rows < 2 * device_cu_count() ? workgroups / n_rows : 1;
+  if (splits > trips) splits = trips;
+  if (splits > kJoinEntries / k) splits = kJoinEntries / k;
+  if (splits < 1) splits = 1;
+  const int64_t each = (trips + splits - 1) / splits;
+  p.splits = (int)((trips + each - 1) / each);
+  p.split_cols = p.splits > 1 ? each * trip : vocab;
+  trips = p.splits > 1 ? each : trips;
+  const int64_t most = kGroupBytes / (int64_t)sizeof(float) / p.threads;  // groups per thread
+  p.span = (int)((trips + most - 1) / most);
+  p.slots = (trips + p.span - 1) / p.span * p.threads;
+  return p;
+}
+
+template <class D, bool VEC, int NT>
+void launch_topk(const TopkArgs& a, int64_t workgroups, size_t lds_bytes, hipStream_t s) {
+  hipLaunchKernelGGL((row_topk_kernel<D, VEC, NT>), dim3((unsigned)workgroups), dim3(NT), lds_bytes, s, a);
+}
+template <class D, bool VEC>
+void launch_divergence(const DivergenceArgs& a, int64_t n_rows, hipStream_t s) {
+  // few long rows: row_softmax.hip's launch_stats()
+  if (n_rows <= device_cu_count() && a.cols * (int64_t)sizeof(typename D::type) >= 64 * 1024)
+    hipLaunchKernelGGL((row_divergence_kernel<D, VEC, kWide>), dim3((unsigned)n_rows), dim3(kWide), 0, s, a);
+  else
+    hipLaunchKernelGGL((row_divergence_kernel<D, VEC, kNarrow>), dim3((unsigned)n_rows), dim3(kNarrow), 0, s, a);
+}
+
+int check_topk(const char* what, const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t ld, int k,
+               float rcp_temperature) {
+  int st = check_rows(what, logits, dtype, n_rows, vocab, ld);
+  if (st != VAMD_OK) return st;
+  VAMD_REQUIRE(vocab < (1ll << 31), "%s: vocab too large", what);
+  VAMD_REQUIRE(k >= 1 && k <= kMaxK, "%s: k is %d, of 1 to %d", what, k, kMaxK);
+  VAMD_REQUIRE(rcp_temperature > 0.f && rcp_temperature < kInf, "%s: temperature must be positive", what);
+  return VAMD_OK;
+}
+
+template <class D>
+int64_t backward_chunks(int64_t vocab) {
+  const int64_t per_wg = (int64_t)kNarrow * D::kVec * D::kBackwardLoads;
+  return (vocab + per_wg - 1) / per_wg;
+}
+int check_backward(const char* what, const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t ld, int k,
+                   float rcp_temperature, const float* stats, const void* d_logits, int64_t ld_out) {
+  const int st = check_topk(what, logits, dtype, n_rows, vocab, ld, k, rcp_temperature);
+  if (st != VAMD_OK) return st;
+  VAMD_REQUIRE(stats && reinterpret_cast<uintptr_t>(stats) % 16 == 0, "%s: stats must be given, 16-byte aligned", what);
+  VAMD_REQUIRE(d_logits && ld_out >= vocab && d_logits != logits, "%s: bad output", what);
+  VAMD_DTYPE_DISPATCH(dtype, D, {
+    VAMD_REQUIRE(n_rows * backward_chunks<D>(vocab) < (1ll << 31), "%s: too many workgroups", what);
+  });
+  return VAMD_OK;
+}
+int entries_backward(EntriesArgs a, int dtype, int64_t n_rows, hipStream_t s) {
+  VAMD_DTYPE_DISPATCH(dtype, D, {
+    const int64_t chunks = backward_chunks<D>(a.cols);
+    a.chunks = (int)chunks;
+    const bool vec = rows_vectorizable<D>(a.logits, a.ld) && rows_vectorizable<D>(a.out, a.ld_out);
+    const bool stream = cached_rows(n_rows, a.ld, sizeof(typename D::type)) < n_rows;
+    void (*const kernels[2][2])(EntriesArgs) = {
+        {row_entries_backward_kernel<D, false, false>, row_entries_backward_kernel<D, false, true>},
+        {row_entries_backward_kernel<D, true, false>, row_entries_backward_kernel<D, true, true>}};
+    hipLaunchKernelGGL(kernels[vec][stream], dim3((unsigned)(n_rows * chunks)), dim3(kNarrow), 0, s, a);
+  });
+  VAMD_LAUNCH_CHECK();
+  return VAMD_OK;
+}
+
+}  // namespace
+}  // namespace vamd
+
+using namespace vamd;
+
+extern "C" size_t vamd_row_topk_workspace_bytes(int64_t n_rows, int64_t vocab, int dtype, int k) {
+  if (n_rows <= 0 || vocab <= 0 || k <= 0 || k > kMaxK) return 0;
+  const TopkPlan p = plan_topk(n_rows, vocab, dtype, k);
+  if (p.splits == 1) return 0;
+  const size_t parts = (size_t)n_rows * p.splits;
+  return align_up(parts * sizeof(float4), 256) + align_up(parts * k * sizeof(uint64_t), 256);
+}
+
+extern "C" int vamd_row_topk(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t ld, const int64_t* labels,
+                             int k, float rcp_temperature, float* logprobs, float* entropy, float* top, int64_t* index,
+                             float* stats, void* workspace, size_t workspace_bytes, void* stream) {
+  int st = check_topk("row_topk", logits, dtype, n_rows, vocab, ld, k, rcp_temperature);
+  if (st != VAMD_OK) return st;
+  VAMD_REQUIRE(k <= vocab, "row_topk: %d alternatives of %lld", k, (long long)vocab);
+  VAMD_REQUIRE(top && index, "row_topk: null output");
+  VAMD_REQUIRE(!logprobs || labels, "row_topk: logprobs need labels");
+  VAMD_REQUIRE(reinterpret_cast<uintptr_t>(stats) % 16 == 0, "row_topk: stats must be 16-byte aligned");
+  const TopkPlan p = plan_topk(n_rows, vocab, dtype, k);
+  const size_t need = vamd_row_topk_workspace_bytes(n_rows, vocab, dtype, k);
+  if (need && (!workspace || workspace_bytes < need)) {
+    set_error("row_topk: workspace %zu bytes, need %zu", workspace_bytes, need);
+    return VAMD_EWORKSPACE;
+  }
+  VAMD_REQUIRE(n_rows * p.splits < (1ll << 31), "row_topk: too many workgroups");
+  TopkArgs a{logits, ld, vocab, labels, k, p.span, rcp_temperature * kLog2e, rcp_temperature, logprobs, entropy, top, index,
+             reinterpret_cast<float4*>(stats), 0, p.splits, p.split_cols, nullptr, nullptr};
+  if (need) {
+    Carver carve(workspace);
+    a.part_state = carve.take<float4>((size_t)n_rows * p.splits);
+    a.part_entry = carve.take<uint64_t>((size_t)n_rows * p.splits * k);
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  VAMD_DTYPE_DISPATCH(dtype, D, {
+    a.cached_rows = cached_rows(n_rows, ld, sizeof(typename D::type));
+    const bool vec = rows_vectorizable<D>(logits, ld);
+    const auto launch = p.threads == kNarrow ? (vec ? launch_topk<D, true, kNarrow> : launch_topk<D, false, kNarrow>)
+                                             : (vec ? launch_topk<D, true, kWide> : launch_topk<D, false, kWide>);
+    launch(a, n_rows * p.splits, p.lds_bytes(), s);
+    if (p.splits > 1) {
+      VAMD_LAUNCH_CHECK();
+      hipLaunchKernelGGL((row_topk_join_kernel<D>), dim3((unsigned)n_rows), dim3(kNarrow),
+                         (size_t)p.splits * k * sizeof(uint64_t), s, a);
+    }
+  });
+  VAMD_LAUNCH_CHECK();
+  return VAMD_OK;
+}
+
+extern "C" int vamd_row_topk_backward(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t ld,
+                                      const int64_t* labels, int k, const int64_t* index, float rcp_temperature,
+                                      const float* stats, const float* d_logprobs, const float* d_entropy,
+                                      const float* d_top, float* row_scratch, void* d_logits, int64_t ld_out, void* stream) {
+  const int st = check_backward("row_topk_backward", logits, dtype, n_rows, vocab, ld, k, rcp_temperature, stats, d_logits, ld_out);
+  if (st != VAMD_OK) return st;
+  VAMD_REQUIRE(row_scratch, "row_topk_backward: null pointer");
+  VAMD_REQUIRE(d_logprobs || d_entropy || d_top, "row_topk_backward: no upstream gradient");
+  VAMD_REQUIRE((!d_logprobs || labels) && (!d_top || index), "row_topk_backward: gradients of log-probs need their tokens");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int entries = d_top ? k : 0;
+  hipLaunchKernelGGL(row_topk_weight_kernel, dim3((unsigned)((n_rows + kNarrow / 64 - 1) / (kNarrow / 64))), dim3(kNarrow), 0,
+                     s, d_logprobs, labels, vocab, d_top, entries, n_rows, row_scratch);
+  VAMD_LAUNCH_CHECK();
+  EntriesArgs a{logits, ld, vocab, 0, entries, index, d_top, reinterpret_cast<const float4*>(stats), row_scratch, nullptr,
+                labels, d_logprobs, d_entropy, rcp_temperature * kLog2e, rcp_temperature, d_logits, ld_out};
+  return entries_backward(a, dtype, n_rows, s);
+}
+
+static int check_divergence(const char* what, int divergence, float beta) {
+  VAMD_REQUIRE(divergence >= VAMD_DIV_FORWARD_KL && divergence <= VAMD_DIV_JSD, "%s: unknown divergence %d", what, divergence);
+  VAMD_REQUIRE(divergence != VAMD_DIV_JSD || (beta > 0.f && beta < 1.f), "%s: beta must lie between 0 and 1", what);
+  return VAMD_OK;
+}
+
+extern "C" int vamd_row_divergence(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t ld,
+                                   const float* teacher_logprobs, const int64_t* teacher_index, int k, int divergence,
+                                   float beta, float rcp_temperature, float* loss, float* stats, float* slope, void* stream) {
+  int st = check_topk("row_divergence", logits, dtype, n_rows, vocab, ld, k, rcp_temperature);
+  if (st != VAMD_OK) return st;
+  if ((st = check_divergence("row_divergence", divergence, beta)) != VAMD_OK) return st;
+  VAMD_REQUIRE(teacher_logprobs && teacher_index && loss, "row_divergence: null pointer");
+  VAMD_REQUIRE(reinterpret_cast<uintptr_t>(stats) % 16 == 0, "row_divergence: stats must be 16-byte aligned");
+  DivergenceArgs a{logits, ld, vocab, teacher_logprobs, teacher_index, k, divergence, beta, rcp_temperature * kLog2e, loss,
+                   reinterpret_cast<float4*>(stats), slope, 0};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  VAMD_DTYPE_DISPATCH(dtype, D, {
+    a.cached_rows = cached_rows(n_rows, ld, sizeof(typename D::type));
+    if (rows_vectorizable<D>(logits, ld)) launch_divergence<D, true>(a, n_rows, s);
+    else launch_divergence<D, false>(a, n_rows, s);
+  });
+  VAMD_LAUNCH_CHECK();
+  return VAMD_OK;
+}
+
+extern "C" int vamd_row_divergence_backward(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t ld,
+                                            const int64_t* teacher_index, int k, float rcp_temperature, const float* stats,
+                                            const float* slope, const float* d_loss, void* d_logits, int64_t ld_out,
+                                            void* stream) {
+  const int st = check_backward("row_divergence_backward", logits, dtype, n_rows, vocab, ld, k, rcp_temperature, stats, d_logits,
+                                ld_out);
+  if (st != VAMD_OK) return st;
+  VAMD_REQUIRE(teacher_index && slope && d_loss, "row_divergence_backward: null pointer");
+  EntriesArgs a{logits, ld, vocab, 0, k, teacher_index, slope, reinterpret_cast<const float4*>(stats), nullptr, d_loss,
+                nullptr, nullptr, nullptr, rcp_temperature * kLog2e, rcp_temperature, d_logits, ld_out};
+  return entries_backward(a, dtype, n_rows, static_cast<hipStream_t>(stream));
+}

@@ -9,6 +9,7 @@
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 #include <torch/csrc/autograd/anomaly_mode.h>
@@ -497,6 +498,219 @@ Tensor entropy_from_logits(const Tensor& logits, bool fp32_output) {
   return row_stats(logits, logit_rows(logits), Tensor(), fp32_output ? at::kFloat : logits.scalar_type(), false).value;
 }
 
+// ---- top alternatives of materialised logits, and their divergence from a teacher's -----------------------------
+// At the end of a backward pass autograd makes the caller's stream wait for those of the leaves' accumulators.  One that an eager
+// graph of the same leaf keeps alive belongs to that graph's stream: under capture the wait records an event of a stream that is
+// not captured, and ending the capture ends the process.
+void refuse_capture_beside_eager_graph(const char* what, const Tensor& input) {
+  if (!input.defined() || !input.is_cuda() || !input.is_leaf() || !input.requires_grad()) return;
+  const c10::DeviceGuard guard(input.device());
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(input);
+  if (!accumulator) return;
+  const auto stream = accumulator->stream();
+  const auto mine = c10::hip::getCurrentHIPStream(input.device().index());
+  TORCH_CHECK(!stream || stream->id() == mine.id(), what, " cannot be captured while an eager graph of the same leaf is alive: "
+              "delete what was computed from it outside the capture");
+}
+void refuse_trace(const char* what) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), what, " cannot be recorded by torch.jit.trace");
+}
+float rcp_temperature(double temperature) {
+  const float rcp = (float)(1.0 / temperature);
+  if (!(temperature > 0.0) || !(rcp > 0.f) || !std::isfinite(rcp))
+    raise_assertion("temperature must be positive, got " + std::to_string(temperature));
+  return rcp;
+}
+std::vector<int64_t> with_last(at::IntArrayRef shape, int64_t last) {
+  auto v = shape.slice(0, shape.size() - 1).vec();
+  v.push_back(last);
+  return v;
+}
+// The gradient that a recorded pass hands back: no function of its own to differentiate.
+Tensor once_differentiable(const Tensor& d, bool records, const variable_list& grads) {
+  if (!records || !d.defined()) return d;
+  for (const Tensor& g : grads)
+    if (g.defined() && g.requires_grad())
+      return torch::autograd::DelayedError(
+          "trying to differentiate twice a function that was marked with @once_differentiable", 1)({d.detach().requires_grad_()})[0];
+  return d;
+}
+Tensor upstream_rows(const Tensor& g, const at::Device& dev) {
+  return g.defined() ? as_f32(g.detach(), dev) : Tensor();
+}
+
+struct Alternatives {
+  Tensor logprobs, entropy, top, index, stats;
+};
+Alternatives row_topk(const Tensor& logits, const Rows& r, const Tensor& labels, int64_t k, float rcp, bool need_grad) {
+  const at::Device dev = logits.device();
+  const c10::DeviceGuard guard(dev);
+  const auto per_row = logits.sizes().slice(0, logits.dim() - 1);
+  const auto options = at::TensorOptions().dtype(at::kFloat).device(dev);
+  const auto wide = with_last(logits.sizes(), k);
+  Alternatives out{labels.defined() ? at::empty(per_row, options) : Tensor(), at::empty(per_row, options),
+                   at::empty(wide, options), at::empty(wide, options.dtype(at::kLong)),
+                   need_grad ? new_f32({r.n(), 4}, dev) : Tensor()};
+  const size_t bytes = vamd_row_topk_workspace_bytes(r.n(), r.vocab(), r.type, (int)k);
+  const Tensor ws = bytes ? at::empty({(int64_t)bytes}, options.dtype(at::kByte)) : Tensor();
+  check(vamd_row_topk(r.data(), r.type, r.n(), r.vocab(), r.ld, labels.defined() ? labels.const_data_ptr<int64_t>() : nullptr,
+                      (int)k, rcp, f32_out(out.logprobs), f32_out(out.entropy), f32_out(out.top),
+                      out.index.mutable_data_ptr<int64_t>(), f32_out(out.stats), ws.defined() ? ws.mutable_data_ptr() : nullptr,
+                      bytes, stream_of(dev)));
+  return out;
+}
+
+class RowTopk : public torch::autograd::Function<RowTopk> {
+ public:
+  // (log-probs of the labels come last: without labels there are three results)
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const std::optional<Tensor>& labels, int64_t k,
+                               double rcp) {
+    const Tensor lab = labels ? label_rows(*labels, logits) : Tensor();
+    const Rows r = logit_rows(logits);
+    const Alternatives out = row_topk(logits, r, lab, k, (float)rcp, true);
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({out.index});
+    ctx->save_for_backward({r.t, lab, out.index, out.stats});
+    ctx->saved_data["logits_shape"] = logits.sizes().vec();
+    ctx->saved_data["rcp"] = rcp;
+    variable_list result{out.entropy, out.top, out.index};
+    if (lab.defined()) result.push_back(out.logprobs);
+    return result;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const bool records = at::GradMode::is_enabled();
+    Tensor d;
+    {
+      at::AutoGradMode no_grad(false);
+      const auto saved = ctx->get_saved_variables();
+      const auto shape = ctx->saved_data["logits_shape"].toIntVector();
+      const Rows r = saved_rows(saved[0], shape);
+      const at::Device dev = r.t.device();
+      const c10::DeviceGuard guard(dev);
+      const Tensor g_ent = upstream_rows(grads[0], dev), g_top = upstream_rows(grads[1], dev),
+                   g_lp = grads.size() > 3 ? upstream_rows(grads[3], dev) : Tensor();
+      if (g_ent.defined() || g_top.defined() || g_lp.defined()) {
+        const Tensor lab = saved[1].defined() ? saved[1].contiguous() : Tensor(), index = saved[2].contiguous(),
+                     stats = saved[3].contiguous(), scratch = new_f32({r.n()}, dev);
+        d = at::empty(shape, r.t.options());
+        check(vamd_row_topk_backward(r.data(), r.type, r.n(), r.vocab(), r.ld,
+                                     lab.defined() ? lab.const_data_ptr<int64_t>() : nullptr, (int)index.size(-1),
+                                     index.const_data_ptr<int64_t>(), (float)ctx->saved_data["rcp"].toDouble(), f32(stats),
+                                     f32(g_lp), f32(g_ent), f32(g_top), f32_out(scratch), d.mutable_data_ptr(), r.vocab(),
+                                     stream_of(dev)));
+      }
+    }
+    return {once_differentiable(d, records, grads), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// (log-probs of the labels or nothing, entropy, the k largest log-probs, their tokens)
+std::tuple<std::optional<Tensor>, Tensor, Tensor, Tensor> topk_logprobs_from_logits(
+    const Tensor& logits, const std::optional<Tensor>& labels, int64_t k, double temperature) {
+  const char* const name = "topk_logprobs_from_logits";
+  refuse_tangents(name, {&logits});
+  refuse_trace(name);
+  const float rcp = rcp_temperature(temperature);
+  if (logits.dim() < 1 || k < 1 || k > VAMD_TOPK_MAX || k > logits.size(-1))
+    raise_assertion("k must be 1 to " + std::to_string(VAMD_TOPK_MAX) + " and at most the vocabulary, got " +
+                    std::to_string(k) + " for logits " + shape_text(logits));
+  if (labels && (at::isFloatingType(labels->scalar_type()) || at::isComplexType(labels->scalar_type())))
+    raise_assertion(std::string("labels must be whole numbers, got ") + c10::toString(labels->scalar_type()));
+  if (wants_gradient(logits)) {
+    refuse_capture_beside_eager_graph(name, logits);
+    const auto out = RowTopk::apply(logits, labels, k, (double)rcp);
+    return {out.size() > 3 ? std::optional<Tensor>(out[3]) : std::nullopt, out[0], out[1], out[2]};
+  }
+  at::AutoGradMode no_grad(false);
+  const Tensor lab = labels ? label_rows(*labels, logits) : Tensor();
+  const Alternatives out = row_topk(logits, logit_rows(logits), lab, k, rcp, false);
+  return {lab.defined() ? std::optional<Tensor>(out.logprobs) : std::nullopt, out.entropy, out.top, out.index};
+}
+
+// A teacher's tokens in the kernels' form.
+struct Teacher {
+  Tensor logprobs, index;  // [rows, k] fp32 and int64
+  int k() const { return (int)index.size(1); }
+};
+Teacher teacher_rows(const Tensor& logprobs, const Tensor& index, at::IntArrayRef rows, const at::Device& dev) {
+  if (logprobs.sizes() != index.sizes() || index.dim() != (int64_t)rows.size() + 1 ||
+      index.sizes().slice(0, rows.size()) != rows)
+    raise_assertion("the teacher's log-probs " + shape_text(logprobs) + " and indices " + shape_text(index) +
+                    " must have the shape of the tokens and one dimension more");
+  const int64_t k = index.size(-1);
+  if (k < 1 || k > VAMD_TOPK_MAX)
+    raise_assertion("a teacher's tokens must be 1 to " + std::to_string(VAMD_TOPK_MAX) + ", got " + std::to_string(k));
+  if (!at::isFloatingType(logprobs.scalar_type())) raise_assertion("the teacher's log-probs must be of a floating type");
+  if (index.scalar_type() != at::kLong && index.scalar_type() != at::kInt)
+    raise_assertion(std::string("the teacher's indices must be int64 or int32, got ") + c10::toString(index.scalar_type()));
+  return {as_f32(logprobs.detach(), dev).reshape({-1, k}), index.to(dev, at::kLong).reshape({-1, k}).contiguous()};
+}
+
+struct DivergenceResult {
+  Tensor loss, stats, slope;
+};
+DivergenceResult row_divergence(const Tensor& logits, const Rows& r, const Teacher& t, int kind, float beta, float rcp,
+                                bool need_grad) {
+  const at::Device dev = logits.device();
+  const c10::DeviceGuard guard(dev);
+  const DivergenceResult out{
+      at::empty(logits.sizes().slice(0, logits.dim() - 1), at::TensorOptions().dtype(at::kFloat).device(dev)),
+      need_grad ? new_f32({r.n(), 4}, dev) : Tensor(), need_grad ? new_f32({r.n(), t.k()}, dev) : Tensor()};
+  check(vamd_row_divergence(r.data(), r.type, r.n(), r.vocab(), r.ld, f32(t.logprobs), t.index.const_data_ptr<int64_t>(), t.k(),
+                            kind, beta, rcp, f32_out(out.loss), f32_out(out.stats), f32_out(out.slope), stream_of(dev)));
+  return out;
+}
+
+class RowDivergence : public torch::autograd::Function<RowDivergence> {
+ public:
+  static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& logprobs, const Tensor& index, int64_t kind,
+                        double beta, double rcp) {
+    const Rows r = logit_rows(logits);
+    const Teacher t = teacher_rows(logprobs, index, logits.sizes().slice(0, logits.dim() - 1), logits.device());
+    const DivergenceResult out = row_divergence(logits, r, t, (int)kind, (float)beta, (float)rcp, true);
+    ctx->save_for_backward({r.t, t.index, out.stats, out.slope});
+    ctx->saved_data["logits_shape"] = logits.sizes().vec();
+    ctx->saved_data["rcp"] = rcp;
+    return out.loss;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const bool records = at::GradMode::is_enabled();
+    Tensor d;
+    {
+      at::AutoGradMode no_grad(false);
+      const auto saved = ctx->get_saved_variables();
+      const auto shape = ctx->saved_data["logits_shape"].toIntVector();
+      const Rows r = saved_rows(saved[0], shape);
+      const at::Device dev = r.t.device();
+      const c10::DeviceGuard guard(dev);
+      const Tensor g = upstream_rows(grads[0], dev), index = saved[1].contiguous(), stats = saved[2].contiguous(),
+                   slope = saved[3].contiguous();
+      d = at::empty(shape, r.t.options());
+      check(vamd_row_divergence_backward(r.data(), r.type, r.n(), r.vocab(), r.ld, index.const_data_ptr<int64_t>(),
+                                         (int)index.size(-1), (float)ctx->saved_data["rcp"].toDouble(), f32(stats), f32(slope),
+                                         f32(g), d.mutable_data_ptr(), r.vocab(), stream_of(dev)));
+    }
+    return {once_differentiable(d, records, grads), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor topk_distillation_from_logits(const Tensor& logits, const Tensor& logprobs, const Tensor& index, int64_t kind,
+                                     double beta, double temperature) {
+  const char* const name = "topk_distillation_from_logits";
+  refuse_tangents(name, {&logits, &logprobs});
+  refuse_trace(name);
+  const float rcp = rcp_temperature(temperature);
+  if (wants_gradient(logits)) {
+    refuse_capture_beside_eager_graph(name, logits);
+    return RowDivergence::apply(logits, logprobs, index, kind, beta, (double)rcp);
+  }
+  at::AutoGradMode no_grad(false);
+  const Rows r = logit_rows(logits);
+  const Teacher t = teacher_rows(logprobs, index, logits.sizes().slice(0, logits.dim() - 1), logits.device());
+  return row_divergence(logits, r, t, (int)kind, (float)beta, rcp, false).loss;
+}
+
 // ---- policy loss ---------------------------------------------------------------------------------------------
 struct PolicyArgs {
   int variant;
@@ -934,6 +1148,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   });
   m.def("logprobs_from_logits", &logprobs_from_logits);
   m.def("entropy_from_logits", &entropy_from_logits);
+  m.def("topk_logprobs_from_logits", &topk_logprobs_from_logits);
+  m.def("topk_distillation_from_logits", &topk_distillation_from_logits);
   m.def("policy_loss", &policy_loss);
   m.def("value_loss", &value_loss);
   m.def("kl_loss", &kl_loss);

@@ -162,6 +162,54 @@ def entropy_from_logits_with_chunking(logits: torch.Tensor, chunk_size: int = 20
     return _native_rows("entropy_from_logits", _EntropyFromLogits, logits, True)
 
 
+def topk_logprobs_from_logits(logits: torch.Tensor, labels: torch.Tensor | None, k: int, temperature: float = 1.0):
+    """``(logprobs, entropy, topk_logprobs, topk_indices)`` of ``softmax(logits / temperature)`` in one pass over the logits.
+
+    ``logprobs`` (of ``labels``; ``None`` without) and ``entropy`` have the shape ``logits.shape[:-1]``, the other two one
+    dimension of ``k`` more: the ``k`` largest logits, largest first, the lowest index first among equals, ``1 <= k <= 256``.
+    fp32 (indices int64) for fp32, bf16 and fp16 logits.  A label outside the vocabulary yields 0.  Logits of ``-inf`` have
+    probability 0: they add nothing to the entropy and come last among the alternatives, with log-probability ``-inf``.  A NaN
+    ranks below them and makes the log-probabilities of its row NaN.  Differentiable once in ``logits``, through all three
+    results."""
+    assert isinstance(k, int), f"k must be an int, but got {type(k)}"
+    if not logits.is_cuda:
+        _logit_rows(logits)   # says what is missing
+    return _cabi.ops().topk_logprobs_from_logits(logits, labels, k, float(temperature))
+
+
+DIVERGENCES = {"forward_kl": 0, "reverse_kl": 1, "jsd": 2}   # VAMD_DIV_*
+
+
+def divergence_code(divergence: str, beta: float) -> int:
+    if divergence not in DIVERGENCES:
+        raise ValueError(f"Invalid divergence: {divergence}, must be one of {list(DIVERGENCES)}")
+    if divergence == "jsd":
+        assert 0.0 < beta < 1.0, f"beta must lie between 0 and 1, but got {beta}"
+    return DIVERGENCES[divergence]
+
+
+def topk_distillation_from_logits(logits: torch.Tensor, teacher_logprobs: torch.Tensor, teacher_indices: torch.Tensor,
+                                  divergence: str = "forward_kl", beta: float = 0.5, temperature: float = 1.0) -> torch.Tensor:
+    """Divergence of ``q = softmax(logits / temperature)`` from a teacher's most likely tokens, per token: fp32 of the shape
+    ``logits.shape[:-1]``, to be aggregated like any per-token loss (``agg_loss``).
+
+    ``teacher_logprobs`` ``t`` and ``teacher_indices`` (int64 or int32), one dimension of 1 to 256 tokens more than that: what
+    ``topk_logprobs_from_logits`` returns for the teacher's logits at the same temperature.  With ``p = exp(t)``, sums over these
+    tokens and ``q`` normalised over the whole vocabulary:
+
+    * ``"forward_kl"``: ``sum p (t - log q)``;
+    * ``"reverse_kl"``: ``sum q (log q - t)``;
+    * ``"jsd"``: ``beta sum p (t - log m) + (1 - beta) sum q (log q - log m)`` with ``m = beta p + (1 - beta) q``.
+
+    An entry whose index lies outside the vocabulary (padding, such as -1) or whose log-probability is ``-inf`` adds nothing; an
+    index that comes twice counts twice.  Differentiable once in ``logits``; the teacher gets no gradient."""
+    code = divergence_code(divergence, beta)
+    if not logits.is_cuda:
+        _logit_rows(logits)   # says what is missing
+    return _cabi.ops().topk_distillation_from_logits(logits, teacher_logprobs, teacher_indices, code, float(beta),
+                                                     float(temperature))
+
+
 class _ClipByValue(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, tensor_min, tensor_max):
