@@ -278,6 +278,29 @@ int vamd_row_divergence(const void* logits, int dtype, int64_t n_rows, int64_t v
 int vamd_row_divergence_backward(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t ld,
                                  const int64_t* teacher_index, int k, float rcp_temperature, const float* stats,
                                  const float* slope, const float* d_loss, void* d_logits, int64_t ld_out, void* stream);
+/* The same two from the head's hidden states [n_tokens, hidden_size] and weight [vocab, hidden_size] (bf16), with the shapes,
+ * labels and results of vamd_lce_forward.
+ * vamd_lce_topk: logprobs, entropy, top and index as vamd_row_topk's, of the fp32 products hidden . weight; the logits of
+ *   token_chunk tokens at a time (0: a few thousand) lie in the workspace.
+ * vamd_lce_divergence: the loss, for the lse (and the logits cache, or NULL) of a vamd_lce_forward call at the same temperature;
+ *   slope_sum [n_tokens], slope and prob [n_tokens, k] (fp32) are what the backward pass needs, NULL together without one.
+ * vamd_lce_divergence_backward: vamd_lce_backward_subset_rows for d_loss [n_tokens] and d_loss_slope = d_loss * slope_sum;
+ *   no_labels: int64 [n_tokens], all -1. */
+size_t vamd_lce_topk_workspace_bytes(int64_t n_tokens, int64_t hidden_size, int64_t vocab, int k, int64_t token_chunk);
+int vamd_lce_topk(const void* hidden, const void* weight, const int64_t* labels, int64_t n_tokens, int64_t hidden_size,
+                  int64_t vocab, int k, float rcp_temperature, float* logprobs, float* entropy, float* top, int64_t* index,
+                  int64_t token_chunk, void* workspace, size_t workspace_bytes, void* stream);
+int vamd_lce_divergence(const void* hidden, const void* weight, const float* logits_cache, int64_t n_tokens,
+                        int64_t hidden_size, int64_t vocab, const float* teacher_logprobs, const int64_t* teacher_index, int k,
+                        int divergence, float beta, float rcp_temperature, const float* lse, float* loss, float* slope_sum,
+                        float* slope, float* prob, void* stream);
+int vamd_lce_divergence_backward(const void* hidden, const void* weight, const int64_t* no_labels, int64_t n_tokens,
+                                 int64_t planned_tokens, int64_t hidden_size, int64_t vocab, const int64_t* teacher_index,
+                                 int k, float rcp_temperature, const float* lse, const float* slope_sum, const float* slope,
+                                 const float* prob, const float* d_loss, const float* d_loss_slope, const float* logits_cache,
+                                 const int64_t* logits_rows, void* d_hidden, void* d_weight, int d_weight_mode,
+                                 float* d_weight_acc32, int64_t vocab_chunk, void* workspace, size_t workspace_bytes,
+                                 void* stream);
 /* clip_by_value (verl/utils/torch_functional.py:203-221): out = max(min(x, hi), lo) over n fp32 elements, and its
  * gradients with torch's rule for binary min / max (the selected operand takes the gradient, equal operands half
  * each); d_x / d_lo / d_hi may be NULL.  A NaN in x, lo or hi gives a NaN output, as torch.min / torch.max of two

@@ -79,6 +79,15 @@ SIGNATURES = {
                                     c_float, c_void_p, c_void_p, c_void_p, c_void_p]),
     "vamd_row_divergence_backward": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int, c_float, c_void_p,
                                              c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "vamd_lce_topk_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int, c_int64]),
+    "vamd_lce_topk": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_float, c_void_p, c_void_p,
+                              c_void_p, c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
+    "vamd_lce_divergence": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int,
+                                    c_float, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "vamd_lce_divergence_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int,
+                                             c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                             c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_size_t,
+                                             c_void_p]),
     "vamd_clip_by_value": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
     "vamd_clip_by_value_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
                                             c_void_p, c_void_p]),

@@ -18,7 +18,7 @@ LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libverl_amd.so")
 OPS_PATH = os.path.join(LIB_DIR, "_torch_ops.so")
 SOURCES = ["runtime.hip", "lce.hip", "policy_math.hip", "gae.hip", "returns_scan.hip", "otb.hip", "metrics.hip", "rollout_corr.hip", "response_window.hip", "cov_select.hip", "row_softmax.hip", "row_topk.hip"]
-HEADERS = ["common.h", "gemm_core.h", "rowchunk.h", "logit_rows.h", os.path.join("..", "..", "include", "verl_amd.h")]
+HEADERS = ["common.h", "gemm_core.h", "rowchunk.h", "logit_rows.h", "divergence.h", os.path.join("..", "..", "include", "verl_amd.h")]
 
 OPS_SOURCE = "torch_ops.cpp"   # host code only: torch's C++ interface over the C ABI
 

@@ -19,6 +19,7 @@
 #include <vector>
 
 #include "common.h"
+#include "divergence.h"
 #include "gemm_core.h"
 
 namespace vamd {
@@ -152,7 +153,9 @@ struct FwdArgs {
   float scale2;      // log2(e) / temperature
   float rcp_t;       // 1 / temperature
   float4* partials;  // [plan.slots()][256] : (max in the log2 domain, sum e, sum e x with x = hidden . weight, label logit)
-  float* z_cache;    // optional [n_tokens][vocab] fp32 logits / temperature, kept for the backward
+  float* z_cache;    // optional [n_tokens][z_ld] fp32 products times z_scale: logits / temperature, kept for the backward
+  int64_t z_ld;      // a multiple of 4; columns from vocab up to the next multiple of 4 are overwritten
+  float z_scale;
   float* pi2_partials;  // optional [plan.slots()][256] : sum of e^2 relative to the same max
   int stream_from;      // lce_forward_few_kernel: stream_from()
 };
@@ -454,13 +457,15 @@ struct FwdEpi {
   __device__ __forceinline__ void store_logits(const Accum& acc, int r0, int c0) {
     const int tok0 = r0 + p.wr * (kNB * kBlk), n_tokens = args->n_tokens;
     float* const z_cache = args->z_cache;
+    const int64_t z_ld = args->z_ld;
+    const float z_scale = args->z_scale;
     CacheExchange ex;
     ex.init(patches, p);
 #pragma unroll
     for (int nb = 0; nb < kNB; ++nb)
 #pragma unroll
       for (int mb2 = 0; mb2 < kMB2; ++mb2) {
-        const f32x4 blk[2][1] = {{acc.a[2 * mb2][nb] * rcp_t}, {acc.a[2 * mb2 + 1][nb] * rcp_t}};
+        const f32x4 blk[2][1] = {{acc.a[2 * mb2][nb] * z_scale}, {acc.a[2 * mb2 + 1][nb] * z_scale}};
         f32x4 out[2];
         ex.run(blk, out);
         const int col = c0 + p.wc * 128 + mb2 * 32 + 4 * ex.rd_chunk;
@@ -469,7 +474,7 @@ struct FwdEpi {
           for (int i = 0; i < 2; ++i) {
             const int tok = tok0 + nb * kBlk + 8 * i + ex.rd_row;
             if (tok < n_tokens)
-              __builtin_nontemporal_store(out[i], reinterpret_cast<f32x4*>(z_cache + (int64_t)tok * vocab + col));
+              __builtin_nontemporal_store(out[i], reinterpret_cast<f32x4*>(z_cache + (int64_t)tok * z_ld + col));
           }
         }
       }
@@ -718,17 +723,17 @@ __global__ __launch_bounds__(kThreads) void lce_forward_few_kernel(FwdArgs a) {
       for (int nb = 0; nb < kNB; ++nb)
 #pragma unroll
         for (int mb2 = 0; mb2 < kFewMB / 2; ++mb2) {
-          const f32x4 blk[2][1] = {{acc[2 * mb2][nb] * a.rcp_t}, {acc[2 * mb2 + 1][nb] * a.rcp_t}};
+          const f32x4 blk[2][1] = {{acc[2 * mb2][nb] * a.z_scale}, {acc[2 * mb2 + 1][nb] * a.z_scale}};
           f32x4 out[2];
           ex.run(blk, out);
-          // 4 columns that exist or do not: vocab % 8 == 0, and tiles end at multiples of kBlk or at the vocabulary
+          // tiles end at multiples of kBlk or at the vocabulary
           const int col = col0 - 4 * lq + 32 * mb2 + 4 * ex.rd_chunk;
           if (col < tile_end(tile)) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const int tok = wr * (kNB * kBlk) + nb * kBlk + 8 * i + ex.rd_row;
               if (tok < a.n_tokens)
-                __builtin_nontemporal_store(out[i], reinterpret_cast<f32x4*>(a.z_cache + (int64_t)tok * a.vocab + col));
+                __builtin_nontemporal_store(out[i], reinterpret_cast<f32x4*>(a.z_cache + (int64_t)tok * a.z_ld + col));
             }
           }
         }
@@ -1155,6 +1160,115 @@ __global__ __launch_bounds__(256) void lce_dlogits_kernel(DLogitsArgs a) {
     if (j < a.chunk_cols) *reinterpret_cast<u32x2*>(a.dz + (int64_t)tok * a.dz_ld + j) = out[g];
   }
 }
+
+// The entries of a gradient g (sum_k c_k [j = i_k] - q_j sum_k c_k) / T whose second term the panel holds: each is computed again, with
+// every c_k of its column, and rounded once.  A wavefront per token.
+struct PanelEntriesArgs {
+  const int64_t* index;  // [n_tokens][k]
+  const float* slope;    // [n_tokens][k]: c_k
+  const float* prob;     // [n_tokens][k]: q of the column, or -1 for an entry that does not count
+  const float* slope_sum;  // [n_tokens]
+  const float* grad;       // [n_tokens]: g
+  int n_tokens, k;
+  float rcp_t;
+  int64_t chunk_c0, chunk_cols;  // columns of the chunk that exist
+  uint16_t* dz;
+  int dz_ld;
+};
+__global__ __launch_bounds__(256) void lce_panel_entries_kernel(PanelEntriesArgs a) {
+  const int tok = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (tok >= a.n_tokens) return;
+  const int64_t* const index = a.index + (int64_t)tok * a.k;
+  const float* const slope = a.slope + (int64_t)tok * a.k;
+  const float g = a.grad[tok] * a.rcp_t, sum = a.slope_sum[tok];
+  for (int e = lane; e < a.k; e += 64) {
+    const int64_t col = index[e], j = col - a.chunk_c0;
+    const float q = a.prob[(int64_t)tok * a.k + e];
+    if (j < 0 || j >= a.chunk_cols || q < 0.f) continue;
+    float c = 0.f;
+    for (int i = 0; i < a.k; ++i) c += index[i] == col ? slope[i] : 0.f;
+    const __bf16 d = (__bf16)(g * fmaf(-q, sum, c));
+    a.dz[(int64_t)tok * a.dz_ld + j] = __builtin_bit_cast(uint16_t, d);
+  }
+}
+
+// Divergence of a token's softmax from a teacher's tokens, whose logits come from the logits cache, or, where there is none, are formed
+// again from the token's hidden states and the tokens' weight rows.  A workgroup per token; a wavefront per product.
+struct HeadDivergenceArgs {
+  const uint16_t* hidden;
+  const uint16_t* weight;
+  const float* z_cache;  // [n_tokens][vocab] logits / temperature, or null
+  const float* lse;
+  const float* teacher;  // [n_tokens][k] log-probabilities
+  const int64_t* index;  // [n_tokens][k]
+  int64_t vocab;
+  int n_tokens, hidden_size, k, kind;
+  float beta, rcp_t;
+  float* loss;
+  float* slope_sum;  // these may be null together
+  float* slope;
+  float* prob;
+};
+__global__ __launch_bounds__(256) void lce_divergence_kernel(HeadDivergenceArgs a) {
+  __shared__ float z[VAMD_TOPK_MAX];
+  __shared__ float red[2][4];
+  const int tok = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t* const index = a.index + (int64_t)tok * a.k;
+  const float* const teacher = a.teacher + (int64_t)tok * a.k;
+  const auto counts = [&](int e) { return index[e] >= 0 && index[e] < a.vocab && teacher[e] != -__builtin_huge_valf(); };
+  if (a.z_cache) {
+    for (int e = threadIdx.x; e < a.k; e += 256) z[e] = counts(e) ? a.z_cache[(int64_t)tok * a.vocab + index[e]] : 0.f;
+  } else {
+    const u32x4* const h = reinterpret_cast<const u32x4*>(a.hidden + (int64_t)tok * a.hidden_size);
+    for (int e = w; e < a.k; e += 4) {
+      float sum = 0.f;
+      if (counts(e)) {
+        const u32x4* const row = reinterpret_cast<const u32x4*>(a.weight + index[e] * a.hidden_size);
+        for (int i = lane; i < a.hidden_size / 8; i += 64) {
+          const u32x4 x = h[i], y = row[i];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            sum = fmaf(bf16_bits_to_float(x[j] & 0xffffu), bf16_bits_to_float(y[j] & 0xffffu), sum);
+            sum = fmaf(bf16_bits_to_float(x[j] >> 16), bf16_bits_to_float(y[j] >> 16), sum);
+          }
+        }
+      }
+#pragma unroll
+      for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+      if (lane == 0) z[e] = sum * a.rcp_t;
+    }
+  }
+  __syncthreads();
+  const int e = threadIdx.x;  // VAMD_TOPK_MAX entries at most
+  Term mine{0.f, 0.f};
+  if (e < a.k) {
+    float q = -1.f;
+    if (counts(e)) {
+      const float log_q = z[e] - a.lse[tok];
+      mine = divergence_term(a.kind, a.beta, teacher[e], log_q);
+      q = expf(log_q);
+    }
+    if (a.slope) {
+      a.slope[(int64_t)tok * a.k + e] = mine.slope;
+      a.prob[(int64_t)tok * a.k + e] = q;
+    }
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    mine.loss += __shfl_xor(mine.loss, off, 64);
+    mine.slope += __shfl_xor(mine.slope, off, 64);
+  }
+  if (lane == 0) {
+    red[0][w] = mine.loss;
+    red[1][w] = mine.slope;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    a.loss[tok] = red[0][0] + red[0][1] + red[0][2] + red[0][3];
+    if (a.slope_sum) a.slope_sum[tok] = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+  }
+}
+static_assert(VAMD_TOPK_MAX <= 256, "an entry per thread");
 
 // ---------------------------------------------------------------------------------------------
 // d_hidden (+)= dz_panel . W[chunk]          R = dz (direct), C = W (kmajor, k = vocab)
@@ -1706,8 +1820,8 @@ extern "C" size_t vamd_lce_forward_workspace_bytes(int64_t n_tokens, int64_t hid
 static int lce_forward_launch(const void* hidden, const void* weight, const int64_t* labels, int64_t n_tokens,
                               int64_t hidden_size, int64_t vocab, float rcp_temperature, float* logprobs,
                               float* entropy, float* lse, float* mean_z, float* logits_cache, float* sum_pi_squared,
-                              void* workspace, void* stream, int64_t max_slots = INT64_MAX) {
-
+                              void* workspace, void* stream, int64_t max_slots = INT64_MAX, int64_t z_ld = 0,
+                              float z_scale = 0.f) {
   FwdArgs a;
   a.hidden = Operand{static_cast<const uint16_t*>(hidden), hidden_size, (int)n_tokens, (int)hidden_size};
   a.weight = Operand{static_cast<const uint16_t*>(weight), hidden_size, (int)vocab, (int)hidden_size};
@@ -1724,6 +1838,8 @@ static int lce_forward_launch(const void* hidden, const void* weight, const int6
                                                   (size_t)a.plan.slots() * kTile * sizeof(float4))
                        : nullptr;
   a.z_cache = logits_cache;
+  a.z_ld = z_ld ? z_ld : vocab;
+  a.z_scale = z_ld ? z_scale : rcp_temperature;
   a.stream_from = stream_from(hidden_size, vocab);
   hipStream_t s = static_cast<hipStream_t>(stream);
   {
@@ -1903,14 +2019,13 @@ extern "C" int vamd_lce_backward_subset(const void* hidden, const void* weight, 
                                        vocab_chunk, workspace, workspace_bytes, stream);
 }
 
-extern "C" int vamd_lce_backward_subset_rows(const void* hidden, const void* weight, const int64_t* labels,
-                                             int64_t n_tokens, int64_t planned_tokens, int64_t hidden_size,
-                                             int64_t vocab, float rcp_temperature, const float* lse,
-                                             const float* mean_z, const float* d_logprobs, const float* d_entropy,
-                                             float d_entropy_scalar, const float* logits_cache,
-                                             const int64_t* logits_rows, void* d_hidden, void* d_weight,
-                                             int d_weight_mode, float* d_weight_acc32, int64_t vocab_chunk,
-                                             void* workspace, size_t workspace_bytes, void* stream) {
+// `entries`: what is added to the panel of each chunk, or null.
+static int lce_backward(const void* hidden, const void* weight, const int64_t* labels, int64_t n_tokens, int64_t planned_tokens,
+                        int64_t hidden_size, int64_t vocab, float rcp_temperature, const float* lse, const float* mean_z,
+                        const float* d_logprobs, const float* d_entropy, float d_entropy_scalar, const float* logits_cache,
+                        const int64_t* logits_rows, void* d_hidden, void* d_weight, int d_weight_mode, float* d_weight_acc32,
+                        int64_t vocab_chunk, void* workspace, size_t workspace_bytes, void* stream,
+                        const PanelEntriesArgs* entries) {
   int st = check_head_shapes(n_tokens, hidden_size, vocab, logits_cache);
   if (st != VAMD_OK) return st;
   VAMD_REQUIRE(hidden && weight && labels && lse && mean_z, "lce_backward: null pointer");
@@ -2027,6 +2142,19 @@ extern "C" int vamd_lce_backward_subset_rows(const void* hidden, const void* wei
       }
     }
 
+    if (entries) {
+      PanelEntriesArgs e = *entries;
+      e.chunk_c0 = c0;
+      e.chunk_cols = cols;
+      e.dz = dz;
+      e.dz_ld = (int)pitch;
+      {
+        ScopedTiming tm(kTagDLogits, s);
+        hipLaunchKernelGGL(lce_panel_entries_kernel, dim3((unsigned)ceil_div(n_tokens, 4)), dim3(256), 0, s, e);
+      }
+      VAMD_LAUNCH_CHECK();
+    }
+
     // d_hidden: k runs over the chunk's vocabulary columns (staged zeros beyond `cols`)
     GemmOutArgs gh;
     // (the panel has no rows past n_tokens: they read as zero through the operand's bounds)
@@ -2089,6 +2217,126 @@ extern "C" int vamd_lce_backward_subset_rows(const void* hidden, const void* wei
                          elements, static_cast<uint16_t*>(d_hidden));
     }
     VAMD_LAUNCH_CHECK();
+  }
+  return VAMD_OK;
+}
+
+extern "C" int vamd_lce_backward_subset_rows(const void* hidden, const void* weight, const int64_t* labels,
+                                             int64_t n_tokens, int64_t planned_tokens, int64_t hidden_size,
+                                             int64_t vocab, float rcp_temperature, const float* lse,
+                                             const float* mean_z, const float* d_logprobs, const float* d_entropy,
+                                             float d_entropy_scalar, const float* logits_cache,
+                                             const int64_t* logits_rows, void* d_hidden, void* d_weight,
+                                             int d_weight_mode, float* d_weight_acc32, int64_t vocab_chunk,
+                                             void* workspace, size_t workspace_bytes, void* stream) {
+  return lce_backward(hidden, weight, labels, n_tokens, planned_tokens, hidden_size, vocab, rcp_temperature, lse, mean_z,
+                      d_logprobs, d_entropy, d_entropy_scalar, logits_cache, logits_rows, d_hidden, d_weight, d_weight_mode,
+                      d_weight_acc32, vocab_chunk, workspace, workspace_bytes, stream, nullptr);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Divergence from a teacher's tokens
+extern "C" int vamd_lce_divergence(const void* hidden, const void* weight, const float* logits_cache, int64_t n_tokens,
+                                   int64_t hidden_size, int64_t vocab, const float* teacher_logprobs,
+                                   const int64_t* teacher_index, int k, int divergence, float beta, float rcp_temperature,
+                                   const float* lse, float* loss, float* slope_sum, float* slope, float* prob, void* stream) {
+  int st = check_head_shapes(n_tokens, hidden_size, vocab, logits_cache);
+  if (st != VAMD_OK) return st;
+  if ((st = check_divergence("lce_divergence", k, divergence, beta)) != VAMD_OK) return st;
+  VAMD_REQUIRE(hidden && weight && teacher_logprobs && teacher_index && lse && loss, "lce_divergence: null pointer");
+  VAMD_REQUIRE((slope_sum && slope && prob) || !(slope_sum || slope || prob),
+               "lce_divergence: slope_sum, slope and prob are written together or not at all");
+  VAMD_REQUIRE((reinterpret_cast<uintptr_t>(hidden) | reinterpret_cast<uintptr_t>(weight)) % 16 == 0,
+               "lce_divergence: hidden and weight must be 16-byte aligned");
+  VAMD_REQUIRE(rcp_temperature > 0.f, "lce_divergence: temperature must be positive");
+  const HeadDivergenceArgs a{static_cast<const uint16_t*>(hidden), static_cast<const uint16_t*>(weight), logits_cache, lse,
+                             teacher_logprobs, teacher_index, vocab, (int)n_tokens, (int)hidden_size, k, divergence, beta,
+                             rcp_temperature, loss, slope_sum, slope, prob};
+  hipLaunchKernelGGL(lce_divergence_kernel, dim3((unsigned)n_tokens), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+  VAMD_LAUNCH_CHECK();
+  return VAMD_OK;
+}
+
+extern "C" int vamd_lce_divergence_backward(const void* hidden, const void* weight, const int64_t* no_labels, int64_t n_tokens,
+                                            int64_t planned_tokens, int64_t hidden_size, int64_t vocab,
+                                            const int64_t* teacher_index, int k, float rcp_temperature, const float* lse,
+                                            const float* slope_sum, const float* slope, const float* prob,
+                                            const float* d_loss, const float* d_loss_slope, const float* logits_cache,
+                                            const int64_t* logits_rows, void* d_hidden, void* d_weight, int d_weight_mode,
+                                            float* d_weight_acc32, int64_t vocab_chunk, void* workspace,
+                                            size_t workspace_bytes, void* stream) {
+  VAMD_REQUIRE(teacher_index && slope_sum && slope && prob && d_loss && d_loss_slope, "lce_divergence_backward: null pointer");
+  VAMD_REQUIRE(k >= 1 && k <= VAMD_TOPK_MAX, "lce_divergence_backward: k is %d, of 1 to %d", k, VAMD_TOPK_MAX);
+  PanelEntriesArgs e{};
+  e.index = teacher_index;
+  e.slope = slope;
+  e.prob = prob;
+  e.slope_sum = slope_sum;
+  e.grad = d_loss;
+  e.n_tokens = (int)n_tokens;
+  e.k = k;
+  e.rcp_t = rcp_temperature;
+  // -q_j g sum c / T is what a log-prob of no column with the upstream gradient g sum c leaves (mean_z is read and multiplied by 0)
+  return lce_backward(hidden, weight, no_labels, n_tokens, planned_tokens, hidden_size, vocab, rcp_temperature, lse, lse,
+                      d_loss_slope, nullptr, 0.f, logits_cache, logits_rows, d_hidden, d_weight, d_weight_mode, d_weight_acc32,
+                      vocab_chunk, workspace, workspace_bytes, stream, &e);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Top alternatives: the logits of `token_chunk` tokens at a time are written out in fp32, unscaled, so that their order is that of
+// the products, and the k largest of each row are picked from them.
+static int64_t topk_pitch(int64_t vocab) { return ceil_div(vocab, 4) * 4; }
+static int64_t topk_tokens(int64_t n_tokens, int64_t requested) {
+  if (requested > 0) return requested < n_tokens ? requested : n_tokens;
+  // equal chunks of whole token tiles, at most 6144 tokens (3.7 GB of logits at 152064 columns)
+  const int64_t chunks = ceil_div(n_tokens, 6144), each = ceil_div(ceil_div(n_tokens, chunks), kTile) * kTile;
+  return each < n_tokens ? each : n_tokens;
+}
+
+extern "C" size_t vamd_lce_topk_workspace_bytes(int64_t n_tokens, int64_t hidden_size, int64_t vocab, int k, int64_t token_chunk) {
+  if (n_tokens <= 0 || vocab <= 0) return 0;
+  const int64_t each = topk_tokens(n_tokens, token_chunk), rest = n_tokens % each;
+  size_t forward = vamd_lce_forward_workspace_bytes(each, hidden_size, vocab), rows = vamd_row_topk_workspace_bytes(each, vocab, VAMD_DT_F32, k);
+  if (rest) {
+    const size_t f = vamd_lce_forward_workspace_bytes(rest, hidden_size, vocab), r = vamd_row_topk_workspace_bytes(rest, vocab, VAMD_DT_F32, k);
+    forward = f > forward ? f : forward;
+    rows = r > rows ? r : rows;
+  }
+  return align_up((size_t)each * topk_pitch(vocab) * 4, 256) + align_up(forward, 256) + align_up((size_t)each * 2 * 4, 256) +
+         align_up(rows, 256);
+}
+
+extern "C" int vamd_lce_topk(const void* hidden, const void* weight, const int64_t* labels, int64_t n_tokens,
+                             int64_t hidden_size, int64_t vocab, int k, float rcp_temperature, float* logprobs,
+                             float* entropy, float* top, int64_t* index, int64_t token_chunk, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+  int st = check_head_shapes(n_tokens, hidden_size, vocab, nullptr);
+  if (st != VAMD_OK) return st;
+  VAMD_REQUIRE(hidden && weight && labels && logprobs && entropy && top && index, "lce_topk: null pointer");
+  VAMD_REQUIRE(k >= 1 && k <= VAMD_TOPK_MAX && k <= vocab, "lce_topk: k is %d, of 1 to %d and the vocabulary", k, VAMD_TOPK_MAX);
+  VAMD_REQUIRE(rcp_temperature > 0.f, "lce_topk: temperature must be positive");
+  const size_t need = vamd_lce_topk_workspace_bytes(n_tokens, hidden_size, vocab, k, token_chunk);
+  if (!workspace || workspace_bytes < need) {
+    set_error("lce_topk: workspace %zu bytes, need %zu", workspace_bytes, need);
+    return VAMD_EWORKSPACE;
+  }
+  if ((st = ensure_lds_attributes()) != VAMD_OK) return st;
+  const int64_t each = topk_tokens(n_tokens, token_chunk), pitch = topk_pitch(vocab);
+  for (int64_t t0 = 0; t0 < n_tokens; t0 += each) {
+    const int64_t n = n_tokens - t0 < each ? n_tokens - t0 : each;
+    Carver carve(workspace);
+    float* const z = carve.take<float>((size_t)each * pitch);
+    float* const lse = carve.take<float>((size_t)each * 2);
+    void* const forward = carve.take<char>(vamd_lce_forward_workspace_bytes(n, hidden_size, vocab));
+    const size_t row_bytes = vamd_row_topk_workspace_bytes(n, vocab, VAMD_DT_F32, k);
+    void* const rows = carve.take<char>(row_bytes);
+    st = lce_forward_launch(static_cast<const uint16_t*>(hidden) + t0 * hidden_size, weight, labels + t0, n, hidden_size, vocab,
+                            rcp_temperature, logprobs + t0, entropy + t0, lse, lse + each, z, nullptr, forward, stream,
+                            INT64_MAX, pitch, 1.f);
+    if (st != VAMD_OK) return st;
+    st = vamd_row_topk(z, VAMD_DT_F32, n, vocab, pitch, nullptr, k, rcp_temperature, nullptr, nullptr, top + t0 * k,
+                       index + t0 * k, nullptr, rows, row_bytes, stream);
+    if (st != VAMD_OK) return st;
   }
   return VAMD_OK;
 }

@@ -13,6 +13,7 @@
 //     -g q_j (z_j - mean) / T^2
 // Bound by HBM: the logits are read once, backward read and written once.
 #include "common.h"
+#include "divergence.h"
 #include "logit_rows.h"
 
 namespace vamd {
@@ -459,30 +460,6 @@ __global__ __launch_bounds__(kNarrow) void row_topk_join_kernel(TopkArgs a) {
 }
 
 // ---- divergence from a teacher's tokens -----------------------------------------------------------------------
-struct Term {
-  float loss, slope;  // of a teacher's token, and its derivative with respect to log q
-};
-// Differences of logarithms are formed from d = log q - t, so that nothing cancels where the two agree.
-__device__ __forceinline__ Term divergence_term(int kind, float beta, float t, float lq) {
-  const float p = expf(t), q = expf(lq), d = lq - t;
-  if (kind == VAMD_DIV_FORWARD_KL) return Term{p > 0.f ? -p * d : 0.f, -p};
-  if (kind == VAMD_DIV_REVERSE_KL) {
-    const float x = q == 0.f ? 0.f : q * d;
-    return Term{x, x + q};
-  }
-  // t - log w and log q - log w
-  float a, b;
-  if (d > 0.f) {
-    b = -log1pf(beta * expm1f(-d));
-    a = b - d;
-  } else {
-    a = -log1pf((1.f - beta) * expm1f(d));
-    b = d + a;
-  }
-  const float x = q == 0.f ? 0.f : (1.f - beta) * q * b;
-  return Term{(p == 0.f ? 0.f : beta * p * a) + x, x};
-}
-
 struct DivergenceArgs {
   const void* logits;
   int64_t ld, cols;
@@ -822,18 +799,12 @@ extern "C" int vamd_row_topk_backward(const void* logits, int dtype, int64_t n_r
   return entries_backward(a, dtype, n_rows, s);
 }
 
-static int check_divergence(const char* what, int divergence, float beta) {
-  VAMD_REQUIRE(divergence >= VAMD_DIV_FORWARD_KL && divergence <= VAMD_DIV_JSD, "%s: unknown divergence %d", what, divergence);
-  VAMD_REQUIRE(divergence != VAMD_DIV_JSD || (beta > 0.f && beta < 1.f), "%s: beta must lie between 0 and 1", what);
-  return VAMD_OK;
-}
-
 extern "C" int vamd_row_divergence(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t ld,
                                    const float* teacher_logprobs, const int64_t* teacher_index, int k, int divergence,
                                    float beta, float rcp_temperature, float* loss, float* stats, float* slope, void* stream) {
   int st = check_topk("row_divergence", logits, dtype, n_rows, vocab, ld, k, rcp_temperature);
   if (st != VAMD_OK) return st;
-  if ((st = check_divergence("row_divergence", divergence, beta)) != VAMD_OK) return st;
+  if ((st = check_divergence("row_divergence", k, divergence, beta)) != VAMD_OK) return st;
   VAMD_REQUIRE(teacher_logprobs && teacher_index && loss, "row_divergence: null pointer");
   VAMD_REQUIRE(reinterpret_cast<uintptr_t>(stats) % 16 == 0, "row_divergence: stats must be 16-byte aligned");
   DivergenceArgs a{logits, ld, vocab, teacher_logprobs, teacher_index, k, divergence, beta, rcp_temperature * kLog2e, loss,

@@ -1148,6 +1148,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   });
   m.def("logprobs_from_logits", &logprobs_from_logits);
   m.def("entropy_from_logits", &entropy_from_logits);
+  m.def("refuse_capture_beside_eager_graph", [](const std::string& what, const Tensor& input) {
+    refuse_capture_beside_eager_graph(what.c_str(), input);
+  });
   m.def("topk_logprobs_from_logits", &topk_logprobs_from_logits);
   m.def("topk_distillation_from_logits", &topk_distillation_from_logits);
   m.def("policy_loss", &policy_loss);
