@@ -21,6 +21,7 @@
 #include "common.h"
 #include "divergence.h"
 #include "gemm_core.h"
+#include "head_pick.h"
 
 namespace vamd {
 
@@ -158,6 +159,8 @@ struct FwdArgs {
   float z_scale;
   float* pi2_partials;  // optional [plan.slots()][256] : sum of e^2 relative to the same max
   int stream_from;      // lce_forward_few_kernel: stream_from()
+  float* group_max;     // kAlternatives: [n_tokens][group_ld], group 8 * (vocabulary tile) + 4 wc + lq
+  int64_t group_ld;
 };
 
 // The tiles of one workgroup.  The ways of sharing out are kernels of their own: with both in one kernel the split
@@ -331,12 +334,18 @@ __device__ __forceinline__ void merge_state(float& m, float& s, float& sy, float
   m = mm;
 }
 
+// What a forward launch is for.  The running sums of kLogprobs take up one term after the other; the others sum a tile's terms first,
+// which keeps a digit more of sums of thousands of terms, at the same number of operations: the log-prob of
+// linear_cross_entropy keeps its bits, and a divergence, a difference of log-probs, gets the digit it loses.
+// kAlternatives also writes the largest product of each lane's 32 columns of a tile.
+enum Purpose : int { kLogprobs = 0, kDivergence = 1, kAlternatives = 2 };
+
 // Per-lane online-softmax state for the kNB token slots (nb) the lane owns.  With CACHE the
 // scaled logits of every valid (token, vocabulary column) are also written out in fp32, so the
 // backward pass can form d_logits without repeating the GEMM.
 // With PI2 a fifth running sum, sum_j e_j^2, is carried, from which sum_j softmax(z)_j^2 follows
 // (calculate_sum_pi_squared_from_logits, verl/utils/torch_functional.py:680-694).
-template <bool CACHE, bool PI2, Walk WALK>
+template <bool CACHE, bool PI2, Walk WALK, Purpose WHY>
 struct FwdEpi {
   LanePos p;
   float scale2;
@@ -523,11 +532,16 @@ struct FwdEpi {
         const lds_f32_t slot = (lds_f32_t)(uintptr_t)(zl_lds + 4u * (threadIdx.x * kNB + nb));
         *slot += add;
       }
+      if constexpr (WHY == kAlternatives) {
+        const int tok = r0 + acc_row(p, nb);
+        if (tok < args->n_tokens) args->group_max[(int64_t)tok * args->group_ld + (c0 >> 5) + 4 * p.wc + p.lq] = xmax;
+      }
       // pass 2: the running state in the log2 domain, three operations and an exponential per element:
       // e = 2^(x scale2 - m), s += e, sy += e x (the raw product: the 1 / temperature goes on at the very end)
       const float m_new = fmaxf(m[nb], xmax * scale2);
       const float resc = fast_exp2(m[nb] - m_new);
-      float s_ = s[nb] * resc, sy_ = sy[nb] * resc, s2_ = PI2 ? s2[nb] * resc * resc : 0.f;
+      constexpr bool kApart = WHY != kLogprobs;
+      float s_ = kApart ? 0.f : s[nb] * resc, sy_ = kApart ? 0.f : sy[nb] * resc, s2_ = PI2 ? s2[nb] * resc * resc : 0.f;
 #pragma unroll
       for (int mb = 0; mb < kMB; ++mb)
 #pragma unroll
@@ -539,20 +553,20 @@ struct FwdEpi {
           if (PI2) s2_ = fmaf(e, e, s2_);
         }
       m[nb] = m_new;
-      s[nb] = s_;
-      sy[nb] = sy_;
+      s[nb] = kApart ? fmaf(s[nb], resc, s_) : s_;
+      sy[nb] = kApart ? fmaf(sy[nb], resc, sy_) : sy_;
       if (PI2) s2[nb] = s2_;
     }
   }
 };
 
-template <bool CACHE, bool PI2, Walk WALK>
+template <bool CACHE, bool PI2, Walk WALK, Purpose WHY>
 __global__ __launch_bounds__(kThreads) void lce_forward_kernel(FwdArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   FwdSched<WALK> sched;
   sched.init(a.plan, a.k_slabs, xcd_regroup(blockIdx.x, gridDim.x));
 
-  FwdEpi<CACHE, PI2, WALK> epi;
+  FwdEpi<CACHE, PI2, WALK, WHY> epi;
   epi.p = lane_pos();
   epi.scale2 = a.scale2;
   epi.vocab = a.vocab;
@@ -620,7 +634,7 @@ __device__ __forceinline__ void few_fetch_weight(const SlabDma<KMAJOR>& dma, con
   }
 }
 
-template <bool CACHE, bool PI2>
+template <bool CACHE, bool PI2, bool APART>
 __global__ __launch_bounds__(kThreads) void lce_forward_few_kernel(FwdArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int split = xcd_regroup(blockIdx.x, gridDim.x);
@@ -755,7 +769,7 @@ __global__ __launch_bounds__(kThreads) void lce_forward_few_kernel(FwdArgs a) {
       zl[nb] += add;
       const float m_new = fmaxf(m[nb], xmax * a.scale2);
       const float resc = fast_exp2(m[nb] - m_new);
-      float s_ = s[nb] * resc, sy_ = sy[nb] * resc, s2_ = PI2 ? s2[nb] * resc * resc : 0.f;
+      float s_ = APART ? 0.f : s[nb] * resc, sy_ = APART ? 0.f : sy[nb] * resc, s2_ = PI2 ? s2[nb] * resc * resc : 0.f;
 #pragma unroll
       for (int mb = 0; mb < kFewMB; ++mb)
 #pragma unroll
@@ -767,8 +781,8 @@ __global__ __launch_bounds__(kThreads) void lce_forward_few_kernel(FwdArgs a) {
           if (PI2) s2_ = fmaf(e, e, s2_);
         }
       m[nb] = m_new;
-      s[nb] = s_;
-      sy[nb] = sy_;
+      s[nb] = APART ? fmaf(s[nb], resc, s_) : s_;
+      sy[nb] = APART ? fmaf(sy[nb], resc, sy_) : sy_;
       if (PI2) s2[nb] = s2_;
     }
   }
@@ -1161,11 +1175,11 @@ __global__ __launch_bounds__(256) void lce_dlogits_kernel(DLogitsArgs a) {
   }
 }
 
-// The entries of a gradient g (sum_k c_k [j = i_k] - q_j sum_k c_k) / T whose second term the panel holds: each is computed again, with
-// every c_k of its column, and rounded once.  A wavefront per token.
+// The entries of a gradient g (sum_k c_k [j = i_k] - q_j sum_k c_k) / T whose second term the panel holds: each is computed again and
+// rounded once.
 struct PanelEntriesArgs {
   const int64_t* index;  // [n_tokens][k]
-  const float* slope;    // [n_tokens][k]: c_k
+  const float* slope;    // [n_tokens][k]: sum of the c of the entry's column
   const float* prob;     // [n_tokens][k]: q of the column, or -1 for an entry that does not count
   const float* slope_sum;  // [n_tokens]
   const float* grad;       // [n_tokens]: g
@@ -1176,20 +1190,15 @@ struct PanelEntriesArgs {
   int dz_ld;
 };
 __global__ __launch_bounds__(256) void lce_panel_entries_kernel(PanelEntriesArgs a) {
-  const int tok = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (tok >= a.n_tokens) return;
-  const int64_t* const index = a.index + (int64_t)tok * a.k;
-  const float* const slope = a.slope + (int64_t)tok * a.k;
-  const float g = a.grad[tok] * a.rcp_t, sum = a.slope_sum[tok];
-  for (int e = lane; e < a.k; e += 64) {
-    const int64_t col = index[e], j = col - a.chunk_c0;
-    const float q = a.prob[(int64_t)tok * a.k + e];
-    if (j < 0 || j >= a.chunk_cols || q < 0.f) continue;
-    float c = 0.f;
-    for (int i = 0; i < a.k; ++i) c += index[i] == col ? slope[i] : 0.f;
-    const __bf16 d = (__bf16)(g * fmaf(-q, sum, c));
-    a.dz[(int64_t)tok * a.dz_ld + j] = __builtin_bit_cast(uint16_t, d);
-  }
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (int64_t)a.n_tokens * a.k) return;
+  const int tok = (int)(i / a.k);
+  const int64_t j = a.index[i] - a.chunk_c0;
+  if (j < 0 || j >= a.chunk_cols) return;
+  const float q = a.prob[i];
+  if (q < 0.f) return;
+  const __bf16 d = (__bf16)(a.grad[tok] * a.rcp_t * fmaf(-q, a.slope_sum[tok], a.slope[i]));
+  a.dz[(int64_t)tok * a.dz_ld + j] = __builtin_bit_cast(uint16_t, d);
 }
 
 // Divergence of a token's softmax from a teacher's tokens, whose logits come from the logits cache, or, where there is none, are formed
@@ -1206,11 +1215,12 @@ struct HeadDivergenceArgs {
   float beta, rcp_t;
   float* loss;
   float* slope_sum;  // these may be null together
-  float* slope;
+  float* slope;      // PanelEntriesArgs
   float* prob;
 };
 __global__ __launch_bounds__(256) void lce_divergence_kernel(HeadDivergenceArgs a) {
-  __shared__ float z[VAMD_TOPK_MAX];
+  __shared__ float z[VAMD_TOPK_MAX];  // later the slopes
+  __shared__ int column[VAMD_TOPK_MAX];
   __shared__ float red[2][4];
   const int tok = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t* const index = a.index + (int64_t)tok * a.k;
@@ -1249,8 +1259,17 @@ __global__ __launch_bounds__(256) void lce_divergence_kernel(HeadDivergenceArgs 
       q = expf(log_q);
     }
     if (a.slope) {
-      a.slope[(int64_t)tok * a.k + e] = mine.slope;
       a.prob[(int64_t)tok * a.k + e] = q;
+      z[e] = mine.slope;
+      column[e] = q < 0.f ? -1 : (int)index[e];
+    }
+  }
+  if (a.slope) {
+    __syncthreads();
+    if (e < a.k) {  // a column that comes several times, in the order of its entries
+      float sum = 0.f;
+      for (int i = 0; i < a.k; ++i) sum += column[i] == column[e] ? z[i] : 0.f;
+      a.slope[(int64_t)tok * a.k + e] = sum;
     }
   }
 #pragma unroll
@@ -1582,14 +1601,24 @@ static int allow_big_lds(K kernel, int bytes = kLdsBytes) {
 typedef void (*ForwardKernel)(FwdArgs);
 // [walk, or few tokens][logits kept][squared sums]
 static const ForwardKernel kForwardKernels[kWalks + 1][2][2] = {
-    {{lce_forward_kernel<false, false, kSplits>, lce_forward_kernel<false, true, kSplits>},
-     {lce_forward_kernel<true, false, kSplits>, lce_forward_kernel<true, true, kSplits>}},
-    {{lce_forward_kernel<false, false, kSplitsIdle>, lce_forward_kernel<false, true, kSplitsIdle>},
-     {lce_forward_kernel<true, false, kSplitsIdle>, lce_forward_kernel<true, true, kSplitsIdle>}},
-    {{lce_forward_kernel<false, false, kBands>, lce_forward_kernel<false, true, kBands>},
-     {lce_forward_kernel<true, false, kBands>, lce_forward_kernel<true, true, kBands>}},
-    {{lce_forward_few_kernel<false, false>, lce_forward_few_kernel<false, true>},
-     {lce_forward_few_kernel<true, false>, lce_forward_few_kernel<true, true>}}};
+    {{lce_forward_kernel<false, false, kSplits, kLogprobs>, lce_forward_kernel<false, true, kSplits, kLogprobs>},
+     {lce_forward_kernel<true, false, kSplits, kLogprobs>, lce_forward_kernel<true, true, kSplits, kLogprobs>}},
+    {{lce_forward_kernel<false, false, kSplitsIdle, kLogprobs>, lce_forward_kernel<false, true, kSplitsIdle, kLogprobs>},
+     {lce_forward_kernel<true, false, kSplitsIdle, kLogprobs>, lce_forward_kernel<true, true, kSplitsIdle, kLogprobs>}},
+    {{lce_forward_kernel<false, false, kBands, kLogprobs>, lce_forward_kernel<false, true, kBands, kLogprobs>},
+     {lce_forward_kernel<true, false, kBands, kLogprobs>, lce_forward_kernel<true, true, kBands, kLogprobs>}},
+    {{lce_forward_few_kernel<false, false, false>, lce_forward_few_kernel<false, true, false>},
+     {lce_forward_few_kernel<true, false, false>, lce_forward_few_kernel<true, true, false>}}};
+// [walk, or few tokens][kDivergence without and with the logits kept, kAlternatives (few tokens: no group maxima)]
+static const ForwardKernel kApartKernels[kWalks + 1][3] = {
+    {lce_forward_kernel<false, false, kSplits, kDivergence>, lce_forward_kernel<true, false, kSplits, kDivergence>,
+     lce_forward_kernel<true, false, kSplits, kAlternatives>},
+    {lce_forward_kernel<false, false, kSplitsIdle, kDivergence>, lce_forward_kernel<true, false, kSplitsIdle, kDivergence>,
+     lce_forward_kernel<true, false, kSplitsIdle, kAlternatives>},
+    {lce_forward_kernel<false, false, kBands, kDivergence>, lce_forward_kernel<true, false, kBands, kDivergence>,
+     lce_forward_kernel<true, false, kBands, kAlternatives>},
+    {lce_forward_few_kernel<false, false, true>, lce_forward_few_kernel<true, false, true>,
+     lce_forward_few_kernel<true, false, true>}};
 
 // The kernels use more LDS than the default launch limit; the limit is a per-device function
 // attribute, so it is raised once on every device the library is used on.
@@ -1607,10 +1636,15 @@ static int ensure_lds_attributes() {
       if ((s = allow_big_lds(kForwardKernels[w][0][pi2], kLdsBytes + kFwdTokenLds)) != VAMD_OK) return s;
       if ((s = allow_big_lds(kForwardKernels[w][1][pi2], kLdsBytes + kFwdCacheLds)) != VAMD_OK) return s;
     }
-  if ((s = allow_big_lds(lce_forward_few_kernel<false, false>, kFewLds)) != VAMD_OK) return s;
-  if ((s = allow_big_lds(lce_forward_few_kernel<false, true>, kFewLds)) != VAMD_OK) return s;
-  if ((s = allow_big_lds(lce_forward_few_kernel<true, false>, kFewCacheLds)) != VAMD_OK) return s;
-  if ((s = allow_big_lds(lce_forward_few_kernel<true, true>, kFewCacheLds)) != VAMD_OK) return s;
+  for (int w = 0; w < kWalks; ++w)
+    for (int i = 0; i < 3; ++i)
+      if ((s = allow_big_lds(kApartKernels[w][i], kLdsBytes + (i ? kFwdCacheLds : kFwdTokenLds))) != VAMD_OK) return s;
+  for (int cache = 0; cache < 2; ++cache) {
+    const int bytes = cache ? kFewCacheLds : kFewLds;
+    if ((s = allow_big_lds(kForwardKernels[kWalks][cache][0], bytes)) != VAMD_OK) return s;
+    if ((s = allow_big_lds(kForwardKernels[kWalks][cache][1], bytes)) != VAMD_OK) return s;
+    if ((s = allow_big_lds(kApartKernels[kWalks][cache], bytes)) != VAMD_OK) return s;
+  }
   if ((s = allow_big_lds(lce_recompute_kernel, kLdsBytes + kRecomputeExtraLds)) != VAMD_OK) return s;
   if ((s = allow_big_lds(lce_dhidden_few_kernel, kFewLds)) != VAMD_OK) return s;
   if ((s = allow_big_lds(lce_dgrad_kernel<false>, kLdsBytes + kGradStageBytes)) != VAMD_OK) return s;
@@ -1820,8 +1854,8 @@ extern "C" size_t vamd_lce_forward_workspace_bytes(int64_t n_tokens, int64_t hid
 static int lce_forward_launch(const void* hidden, const void* weight, const int64_t* labels, int64_t n_tokens,
                               int64_t hidden_size, int64_t vocab, float rcp_temperature, float* logprobs,
                               float* entropy, float* lse, float* mean_z, float* logits_cache, float* sum_pi_squared,
-                              void* workspace, void* stream, int64_t max_slots = INT64_MAX, int64_t z_ld = 0,
-                              float z_scale = 0.f) {
+                              void* workspace, void* stream, int64_t max_slots = INT64_MAX, Purpose why = kLogprobs,
+                              int64_t z_ld = 0, float z_scale = 0.f, float* group_max = nullptr) {
   FwdArgs a;
   a.hidden = Operand{static_cast<const uint16_t*>(hidden), hidden_size, (int)n_tokens, (int)hidden_size};
   a.weight = Operand{static_cast<const uint16_t*>(weight), hidden_size, (int)vocab, (int)hidden_size};
@@ -1840,6 +1874,8 @@ static int lce_forward_launch(const void* hidden, const void* weight, const int6
   a.z_cache = logits_cache;
   a.z_ld = z_ld ? z_ld : vocab;
   a.z_scale = z_ld ? z_scale : rcp_temperature;
+  a.group_max = group_max;
+  a.group_ld = ceil_div(vocab, kTile) * 8;
   a.stream_from = stream_from(hidden_size, vocab);
   hipStream_t s = static_cast<hipStream_t>(stream);
   {
@@ -1849,7 +1885,8 @@ static int lce_forward_launch(const void* hidden, const void* weight, const int6
     const int lds_bytes = a.plan.few_cols ? (cache ? kFewCacheLds : kFewLds) : kLdsBytes + (cache ? kFwdCacheLds : kFwdTokenLds);
     const bool idle = ceil_div(n_tokens, kNB * kBlk) % (kTile / (kNB * kBlk)) != 0;  // a wavefront owns kNB blocks of tokens
     const int walk = a.plan.few_cols ? kWalks : !a.plan.splits ? kBands : idle ? kSplitsIdle : kSplits;
-    hipLaunchKernelGGL(kForwardKernels[walk][cache][pi2], grid, block, lds_bytes, s, a);
+    const ForwardKernel kernel = why == kLogprobs ? kForwardKernels[walk][cache][pi2] : kApartKernels[walk][why == kAlternatives ? 2 : cache];
+    hipLaunchKernelGGL(kernel, grid, block, lds_bytes, s, a);
   }
   VAMD_LAUNCH_CHECK();
 
@@ -2150,7 +2187,7 @@ static int lce_backward(const void* hidden, const void* weight, const int64_t* l
       e.dz_ld = (int)pitch;
       {
         ScopedTiming tm(kTagDLogits, s);
-        hipLaunchKernelGGL(lce_panel_entries_kernel, dim3((unsigned)ceil_div(n_tokens, 4)), dim3(256), 0, s, e);
+        hipLaunchKernelGGL(lce_panel_entries_kernel, dim3((unsigned)ceil_div(n_tokens * e.k, 256)), dim3(256), 0, s, e);
       }
       VAMD_LAUNCH_CHECK();
     }
@@ -2236,6 +2273,25 @@ extern "C" int vamd_lce_backward_subset_rows(const void* hidden, const void* wei
 
 // ---------------------------------------------------------------------------------------------
 // Divergence from a teacher's tokens
+extern "C" int vamd_lce_divergence_forward(const void* hidden, const void* weight, const int64_t* no_labels, int64_t n_tokens,
+                                           int64_t hidden_size, int64_t vocab, float rcp_temperature, float* scratch, float* lse,
+                                           float* logits_cache, void* workspace, size_t workspace_bytes, void* stream) {
+  float* const logprobs = scratch;
+  float* const entropy = scratch ? scratch + n_tokens : nullptr;
+  float* const mean_z = scratch ? scratch + 2 * n_tokens : nullptr;
+  int st = check_forward_args(hidden, weight, no_labels, n_tokens, hidden_size, vocab, rcp_temperature, logprobs, entropy, lse,
+                              mean_z, logits_cache);
+  if (st != VAMD_OK) return st;
+  const size_t need = vamd_lce_forward_workspace_bytes(n_tokens, hidden_size, vocab);
+  if (!workspace || workspace_bytes < need) {
+    set_error("lce_divergence_forward: workspace %zu bytes, need %zu", workspace_bytes, need);
+    return VAMD_EWORKSPACE;
+  }
+  if ((st = ensure_lds_attributes()) != VAMD_OK) return st;
+  return lce_forward_launch(hidden, weight, no_labels, n_tokens, hidden_size, vocab, rcp_temperature, logprobs, entropy, lse,
+                            mean_z, logits_cache, nullptr, workspace, stream, INT64_MAX, kDivergence);
+}
+
 extern "C" int vamd_lce_divergence(const void* hidden, const void* weight, const float* logits_cache, int64_t n_tokens,
                                    int64_t hidden_size, int64_t vocab, const float* teacher_logprobs,
                                    const int64_t* teacher_index, int k, int divergence, float beta, float rcp_temperature,
@@ -2293,17 +2349,23 @@ static int64_t topk_tokens(int64_t n_tokens, int64_t requested) {
   return each < n_tokens ? each : n_tokens;
 }
 
+// Over few tokens, or a vocabulary whose group maxima do not fit into LDS, the rows are read again.
+static bool topk_from_groups(int64_t n_tokens, int64_t vocab) {
+  return n_tokens > kFewTokens && ceil_div(vocab, kTile) * 8 <= kHeadPickGroups;
+}
+// of a chunk of n tokens, behind its logits: partial states, lse and mean_z, group maxima or the rows' own workspace
+static size_t topk_chunk_bytes(int64_t n, int64_t hidden_size, int64_t vocab, int k) {
+  const size_t pick = topk_from_groups(n, vocab) ? (size_t)n * ceil_div(vocab, kTile) * 8 * sizeof(float)
+                                                 : vamd_row_topk_workspace_bytes(n, vocab, VAMD_DT_F32, k);
+  return align_up(vamd_lce_forward_workspace_bytes(n, hidden_size, vocab), 256) + align_up((size_t)n * 2 * sizeof(float), 256) +
+         align_up(pick, 256);
+}
+
 extern "C" size_t vamd_lce_topk_workspace_bytes(int64_t n_tokens, int64_t hidden_size, int64_t vocab, int k, int64_t token_chunk) {
   if (n_tokens <= 0 || vocab <= 0) return 0;
   const int64_t each = topk_tokens(n_tokens, token_chunk), rest = n_tokens % each;
-  size_t forward = vamd_lce_forward_workspace_bytes(each, hidden_size, vocab), rows = vamd_row_topk_workspace_bytes(each, vocab, VAMD_DT_F32, k);
-  if (rest) {
-    const size_t f = vamd_lce_forward_workspace_bytes(rest, hidden_size, vocab), r = vamd_row_topk_workspace_bytes(rest, vocab, VAMD_DT_F32, k);
-    forward = f > forward ? f : forward;
-    rows = r > rows ? r : rows;
-  }
-  return align_up((size_t)each * topk_pitch(vocab) * 4, 256) + align_up(forward, 256) + align_up((size_t)each * 2 * 4, 256) +
-         align_up(rows, 256);
+  const size_t first = topk_chunk_bytes(each, hidden_size, vocab, k), last = rest ? topk_chunk_bytes(rest, hidden_size, vocab, k) : 0;
+  return align_up((size_t)each * topk_pitch(vocab) * sizeof(float), 256) + (first > last ? first : last);
 }
 
 extern "C" int vamd_lce_topk(const void* hidden, const void* weight, const int64_t* labels, int64_t n_tokens,
@@ -2326,16 +2388,22 @@ extern "C" int vamd_lce_topk(const void* hidden, const void* weight, const int64
     const int64_t n = n_tokens - t0 < each ? n_tokens - t0 : each;
     Carver carve(workspace);
     float* const z = carve.take<float>((size_t)each * pitch);
-    float* const lse = carve.take<float>((size_t)each * 2);
     void* const forward = carve.take<char>(vamd_lce_forward_workspace_bytes(n, hidden_size, vocab));
-    const size_t row_bytes = vamd_row_topk_workspace_bytes(n, vocab, VAMD_DT_F32, k);
-    void* const rows = carve.take<char>(row_bytes);
+    float* const lse = carve.take<float>((size_t)n * 2);
+    const bool groups = topk_from_groups(n, vocab);
+    float* const group_max = groups ? carve.take<float>((size_t)n * ceil_div(vocab, kTile) * 8) : nullptr;
     st = lce_forward_launch(static_cast<const uint16_t*>(hidden) + t0 * hidden_size, weight, labels + t0, n, hidden_size, vocab,
-                            rcp_temperature, logprobs + t0, entropy + t0, lse, lse + each, z, nullptr, forward, stream,
-                            INT64_MAX, pitch, 1.f);
+                            rcp_temperature, logprobs + t0, entropy + t0, lse, lse + n, z, nullptr, forward, stream, INT64_MAX,
+                            groups ? kAlternatives : kDivergence, pitch, 1.f, group_max);
     if (st != VAMD_OK) return st;
-    st = vamd_row_topk(z, VAMD_DT_F32, n, vocab, pitch, nullptr, k, rcp_temperature, nullptr, nullptr, top + t0 * k,
-                       index + t0 * k, nullptr, rows, row_bytes, stream);
+    if (groups) {
+      st = launch_head_pick(HeadPickArgs{z, pitch, vocab, group_max, (int)(ceil_div(vocab, kTile) * 8), lse, (int)n, k,
+                                         rcp_temperature, top + t0 * k, index + t0 * k}, static_cast<hipStream_t>(stream));
+    } else {
+      const size_t row_bytes = vamd_row_topk_workspace_bytes(n, vocab, VAMD_DT_F32, k);
+      st = vamd_row_topk(z, VAMD_DT_F32, n, vocab, pitch, nullptr, k, rcp_temperature, nullptr, nullptr, top + t0 * k,
+                         index + t0 * k, nullptr, carve.take<char>(row_bytes), row_bytes, stream);
+    }
     if (st != VAMD_OK) return st;
   }
   return VAMD_OK;

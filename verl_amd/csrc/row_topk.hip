@@ -14,12 +14,13 @@
 // Bound by HBM: the logits are read once, backward read and written once.
 #include "common.h"
 #include "divergence.h"
+#include "head_pick.h"
 #include "logit_rows.h"
 
 namespace vamd {
 namespace {
 
-constexpr int kNarrow = 256, kWide = 1024;  // threads per workgroup
+constexpr int kNarrow = 256, kMiddle = 512, kWide = 1024;  // threads per workgroup
 constexpr int kMaxK = VAMD_TOPK_MAX;
 constexpr float kInf = __builtin_huge_valf();
 
@@ -37,91 +38,177 @@ __device__ __forceinline__ float log_q(float z, float scale2, const Softmax& r) 
   return z < -1.0e30f ? fmaf(z, scale2 * kLn2, -(r.m + log2_s) * kLn2) : (fmaf(z, scale2, -r.m) - log2_s) * kLn2;
 }
 
-// One thread's part of the columns [begin, end).  TOP: beside the softmax state the largest logit of each of the thread's groups,
-// a group being `span` trips of kInFlight 16-byte loads, goes to LDS; `best` is the largest of all.  SUM_Z: whether sz is wanted.
+// what another lane of the row of 16 holds
+template <int CTRL>
+__device__ __forceinline__ float exchanged(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, false));
+}
+
+// A thread's kInFlight groups of logits into its state; returns what they add to sz.  The trip's terms are summed apart and added to
+// the state once: one after the other, the few hundred terms of a thread lose a digit of the sums.  SUM_Z: whether sz is wanted.
+template <bool SUM_Z, int G>
+__device__ __forceinline__ float add_trip(const float (&x)[kInFlight][G], float hi, float scale2, Softmax& st) {
+  const float y = hi * scale2;
+  if (y > st.m) {
+    const float resc = __builtin_amdgcn_exp2f(st.m - y);
+    st.s *= resc;
+    st.sz *= resc;
+    st.m = y;
+  }
+  float s[kInFlight], sz[kInFlight];
+#pragma unroll
+  for (int u = 0; u < kInFlight; ++u) {
+    s[u] = sz[u] = 0.f;
+#pragma unroll
+    for (int e = 0; e < G; ++e) {
+      const float ex = __builtin_amdgcn_exp2f(fmaf(x[u][e], scale2, -st.m));
+      s[u] += ex;
+      if (SUM_Z) sz[u] = fmaf(ex, x[u][e], sz[u]);
+    }
+  }
+  static_assert(kInFlight == 4, "the sums below");
+  st.s += (s[0] + s[1]) + (s[2] + s[3]);
+  return (sz[0] + sz[1]) + (sz[2] + sz[3]);
+}
+// The same sz where a logit is -inf, which adds 0 and not 0 x -inf, or NaN; read again, so that the trip's logits need not be held.
+template <class D>
+__device__ __forceinline__ float sum_with_masked(const typename D::type* row, int64_t c, int64_t stride, int64_t end,
+                                                           float scale2, float m) {
+  float sz = 0.f;
+#pragma unroll 1
+  for (int u = 0; u < kInFlight; ++u, c += stride)
+#pragma unroll 1
+    for (int e = 0; e < D::kVec; ++e) {
+      const float z = c + e < end ? to_float(row[c + e], D()) : -kInf;
+      sz = fmaf(__builtin_amdgcn_exp2f(fmaf(z, scale2, -m)), z == -kInf ? 0.f : z, sz);
+    }
+  return sz;
+}
+
+// What the walk leaves of a thread's trip in LDS: the largest logit, or for 16-bit types, which lose nothing by it, those of the first
+// and of the last two loads, side by side.  A smaller group is less to read again (its loads lie in lines of their own); one of 64
+// bytes in a row, over the lanes of a quad, took ten operations a trip: 4096 x 152064 bf16 k = 5 207 -> 221 us.
+template <class D>
+struct GroupWord {
+  static constexpr int kHalves = sizeof(typename D::type) == 4 ? 1 : 2, kLoads = kInFlight / kHalves;
+  static __device__ __forceinline__ unsigned pack(float a, float b) {
+    if constexpr (std::is_same_v<D, F32>) return __float_as_uint(fmaxf(a, b));
+    else if constexpr (std::is_same_v<D, BF16>) return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+    else return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(a, b));
+  }
+  static __device__ __forceinline__ float half(unsigned word, int i) {
+    if constexpr (std::is_same_v<D, F32>) return __uint_as_float(word);
+    else if constexpr (std::is_same_v<D, BF16>) return __uint_as_float(i ? word & 0xffff0000u : word << 16);
+    else return (float)__builtin_bit_cast(_Float16, (uint16_t)(i ? word >> 16 : word));
+  }
+};
+
+// One thread's part of the columns [begin, end).  TOP: beside the softmax state a word of every `span` trips goes to LDS; `best` is the
+// thread's largest logit.
 template <class D, bool VEC, bool STREAM, int NT, bool TOP, bool SUM_Z>
 __device__ __forceinline__ void walk(const typename D::type* __restrict__ row, int64_t begin, int64_t end, float scale2,
-                                     int span, Softmax& st, float& best, float* groups) {
+                                     int span, Softmax& st, float& best, unsigned* groups) {
   constexpr int G = D::kVec;
-  constexpr int64_t stride = (int64_t)NT * G;
-  float m = kNegBig, s = 0.f, sz = 0.f, held = -kInf;
+  constexpr int64_t stride = (int64_t)NT * G, trip = stride * kInFlight;
+  float held[2] = {-kInf, -kInf};
   int left = span, slot = threadIdx.x;
   best = -kInf;
-  for (int64_t base = begin; base < end; base += stride * kInFlight) {  // the same trips for every thread
-    const int64_t c0 = base + (int64_t)threadIdx.x * G;
-    u32x4_t raw[kInFlight];
-#pragma unroll
-    for (int u = 0; u < kInFlight; ++u) {
-      const int64_t c = c0 + u * stride;
-      if (c + G <= end) raw[u] = load_whole<D, VEC, STREAM>(row + c);
-    }
-    float x[kInFlight][G];
-#pragma unroll
-    for (int u = 0; u < kInFlight; ++u) {
-      const int64_t c = c0 + u * stride;
-      if (c + G <= end) {
-        const Pack<D> p = __builtin_bit_cast(Pack<D>, raw[u]);
-#pragma unroll
-        for (int e = 0; e < G; ++e) x[u][e] = to_float(p.v[e], D());
-      } else {
-        load_ragged<D>(row, c, end, -kInf, x[u]);
-      }
-    }
-    float hi = -kInf, lo = kInf;
+  st = Softmax{kNegBig, 0.f, 0.f};
+  // the trip's largest logit
+  const auto highest = [&](const float (&x)[kInFlight][G], bool last) {
+    float h[2] = {-kInf, -kInf};
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u)
 #pragma unroll
-      for (int e = 0; e < G; ++e) {
-        hi = fmaxf(hi, x[u][e]);
-        if (SUM_Z) lo = fminf(lo, x[u][e]);
-      }
+      for (int e = 0; e < G; ++e) h[u / (kInFlight / 2)] = fmaxf(h[u / (kInFlight / 2)], x[u][e]);
+    const float hi = fmaxf(h[0], h[1]);
     if constexpr (TOP) {
-      held = fmaxf(held, hi);
-      if (--left == 0 || base + stride * kInFlight >= end) {
-        groups[slot] = held;
-        best = fmaxf(best, held);
-        held = -kInf;
+      best = fmaxf(best, hi);
+      held[0] = fmaxf(held[0], h[0]);
+      held[1] = fmaxf(held[1], h[1]);
+      if (--left == 0 || last) {
+        groups[slot] = GroupWord<D>::pack(held[0], held[1]);
+        held[0] = held[1] = -kInf;
         slot += NT;
         left = span;
       }
     }
-    const float y = hi * scale2;
-    if (y > m) {
-      const float resc = __builtin_amdgcn_exp2f(m - y);
-      s *= resc;
-      sz *= resc;
-      m = y;
+    return hi;
+  };
+  const auto add = [&](const float (&x)[kInFlight][G], float hi, int64_t at) {
+    float sz = add_trip<SUM_Z>(x, hi, scale2, st);
+    if constexpr (SUM_Z) {
+      if (__builtin_expect(sz != sz, 0)) sz = sum_with_masked<D>(row, at + (int)threadIdx.x * G, stride, end, scale2, st.m);
+      st.sz += sz;
     }
-    if (SUM_Z && __builtin_expect(lo == -kInf, 0)) {  // masked logits, or none: 2^(-inf) (-inf) is 0 here and not NaN
+  };
+  int64_t base = begin;
+  for (; base + trip <= end; base += trip) {
+    u32x4_t raw[kInFlight];
 #pragma unroll
-      for (int u = 0; u < kInFlight; ++u)
+    for (int u = 0; u < kInFlight; ++u) raw[u] = load_whole<D, VEC, STREAM>(row + base + u * stride + (int)threadIdx.x * G);
+    float x[kInFlight][G];
 #pragma unroll
-        for (int e = 0; e < G; ++e) {
-          const float z = x[u][e];
-          const float ex = z == -kInf ? 0.f : __builtin_amdgcn_exp2f(fmaf(z, scale2, -m));
-          s += ex;
-          sz = fmaf(ex, z == -kInf ? 0.f : z, sz);
-        }
-    } else {
+    for (int u = 0; u < kInFlight; ++u) {
+      const Pack<D> p = __builtin_bit_cast(Pack<D>, raw[u]);
 #pragma unroll
-      for (int u = 0; u < kInFlight; ++u)
-#pragma unroll
-        for (int e = 0; e < G; ++e) {
-          const float z = x[u][e];
-          const float ex = __builtin_amdgcn_exp2f(fmaf(z, scale2, -m));
-          s += ex;
-          if (SUM_Z) sz = fmaf(ex, z, sz);
-        }
+      for (int e = 0; e < G; ++e) x[u][e] = to_float(p.v[e], D());
     }
+    const float hi = highest(x, base + trip >= end);
+    add(x, hi, base);
   }
-  st = Softmax{m, s, sz};
+  if (base < end) {  // the rest: missing logits are -inf, and kNegBig where they are summed
+    const int left_here = (int)(end - base) - (int)threadIdx.x * G;
+    u32x4_t raw[kInFlight];
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u)  // all of them requested first
+      if (left_here - u * (int)stride >= G) raw[u] = load_whole<D, VEC, STREAM>(row + base + u * stride + (int)threadIdx.x * G);
+    float x[kInFlight][G];
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      const int n = left_here - u * (int)stride;
+      if (n >= G) {
+        const Pack<D> p = __builtin_bit_cast(Pack<D>, raw[u]);
+#pragma unroll
+        for (int e = 0; e < G; ++e) x[u][e] = to_float(p.v[e], D());
+      } else {
+#pragma unroll
+        for (int e = 0; e < G; ++e) x[u][e] = -kInf;
+        if (n > 0) load_ragged<D>(row, end - n, end, -kInf, x[u]);
+      }
+    }
+    const float hi = highest(x, true);
+    bool any = false;  // logits other than -inf: without one m may still be kNegBig, and kNegBig no small exponent
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u)
+#pragma unroll
+      for (int e = 0; e < G; ++e) {
+        any = any || x[u][e] != -kInf;
+        if (e >= left_here - u * (int)stride) x[u][e] = kNegBig;
+      }
+    if (any) add(x, hi, base);
+  }
 }
 
-// the wavefront's state in every lane
+// the wavefront's state in every lane: within rows of 16 lanes by moves inside the vector ALU, then the four rows
+template <int CTRL>
+__device__ __forceinline__ void merge_exchanged(Softmax& st) {
+  merge(st, Softmax{exchanged<CTRL>(st.m), exchanged<CTRL>(st.s), exchanged<CTRL>(st.sz)});
+}
+__device__ __forceinline__ Softmax in_lane(const Softmax& st, int lane) {
+  const auto read = [lane](float x) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane)); };
+  return Softmax{read(st.m), read(st.s), read(st.sz)};
+}
 __device__ __forceinline__ void merge_wave(Softmax& st) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1)
-    merge(st, Softmax{__shfl_xor(st.m, off, 64), __shfl_xor(st.s, off, 64), __shfl_xor(st.sz, off, 64)});
+  merge_exchanged<0xB1>(st);   // lane ^ 1
+  merge_exchanged<0x4E>(st);   // lane ^ 2
+  merge_exchanged<0x141>(st);  // the other half of 8
+  merge_exchanged<0x140>(st);  // the other half of 16
+  Softmax a = in_lane(st, 0), b = in_lane(st, 32);
+  merge(a, in_lane(st, 16));
+  merge(b, in_lane(st, 48));
+  merge(a, b);
+  st = a;
 }
 
 // ---- the k largest of a range of a row ------------------------------------------------------------------------
@@ -141,9 +228,9 @@ __device__ __forceinline__ uint64_t entry_of(unsigned order, int64_t col) {
 __device__ __forceinline__ unsigned order_in(uint64_t entry) { return (unsigned)(entry >> 32); }
 __device__ __forceinline__ int64_t column_in(uint64_t entry) { return (int64_t)(0xffffffffu - (unsigned)entry); }
 
-// The walk leaves the maximum of every group in LDS (at most kGroupBytes of them; a row of 152064 bf16 has 4864 groups of 32
-// logits).  The k-th largest of the threads' own maxima is a value that at least k logits reach; only groups that reach it can hold
-// one of the k largest, and these, about k of them, are read again from the caches: k x 64 bytes instead of the row.  What reaches
+// The walk leaves the maximum of every group in LDS (at most kGroupBytes; a row of 152064 bf16 has 4864 words for 9728 groups of
+// 16 logits).  The k-th largest of the threads' own maxima is a value that at least k logits reach; only groups that reach it can hold
+// one of the k largest, and these, about k of them, are read again: k x 2 lines instead of the row.  What reaches
 // the value there, a little more than k logits, is ranked by counting.  Where that list would be too long (many equal logits)
 // the order of the k-th largest is found digit by digit in passes over the row, which is right for any values.
 constexpr int kGroupBytes = 20 * 1024, kGroupList = 512, kCandidates = 1024;
@@ -164,6 +251,7 @@ __device__ __forceinline__ void meet(PickLds<NT>& lds, Softmax st, float best, i
   // bits below it cannot tell two logits of the type apart (fp32: change the value by less than 2^-14)
   constexpr int kLowBit = std::is_same_v<D, BF16> ? 16 : std::is_same_v<D, F16> ? 13 : 9;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int role = (w + (int)blockIdx.x) % (NT / 64);  // every SIMD has one wavefront of each workgroup, so they take turns
   merge_wave(st);
   if (lane == 0) {
     lds.red[0][w] = st.m;
@@ -173,12 +261,12 @@ __device__ __forceinline__ void meet(PickLds<NT>& lds, Softmax st, float best, i
   lds.top[threadIdx.x] = order_of(best);
   if (threadIdx.x == 0) lds.groups = lds.candidates = 0;
   __syncthreads();
-  if (w == 1) {
+  if (role == 1) {
     Softmax all{lds.red[0][0], lds.red[1][0], lds.red[2][0]};
 #pragma unroll
     for (int j = 1; j < NT / 64; ++j) merge(all, Softmax{lds.red[0][j], lds.red[1][j], lds.red[2][j]});
     if (lane == 0) lds.whole = all;
-  } else if (w == 0) {
+  } else if (role == 0) {
     constexpr int P = NT / 64;
     unsigned mine[P];
 #pragma unroll
@@ -201,15 +289,43 @@ __device__ __forceinline__ void meet(PickLds<NT>& lds, Softmax st, float best, i
   __syncthreads();
 }
 
-// emit(rank, entry) for each entry of the list that is among its k largest
+// emit(rank, entry) for each entry of the list that is among its k largest.  A short list is ranked by counting, which reads it once
+// per wavefront of entries (all lanes the same words, at the speed of 64 different ones); a longer one is sorted, by exchanges
+// between entries a power of two apart: 64 x 152064 bf16, k = 256, lists of 400 to 900, 120 us by counting.
+// The list has room for the next power of two; every thread comes here with the list complete.
+constexpr int kCountedList = 192;
 template <int NT, class Emit>
-__device__ __forceinline__ void rank_list(const uint64_t* list, int n, int k, Emit&& emit) {
-  for (int j = threadIdx.x; j < n; j += NT) {
-    const uint64_t mine = list[j];
-    int rank = 0;
-    for (int i = 0; i < n; ++i) rank += list[i] > mine;
-    if (rank < k) emit(rank, mine);
+__device__ __forceinline__ void rank_list(uint64_t* list, int n, int k, Emit&& emit) {
+  if (n <= kCountedList) {
+    for (int j = (threadIdx.x + 64u * blockIdx.x) % NT; j < n; j += NT) {
+      const uint64_t mine = list[j];
+      int rank = 0, i = 0;
+      for (; i + 8 <= n; i += 8) {  // eight reads in flight
+#pragma unroll
+        for (int u = 0; u < 8; ++u) rank += list[i + u] > mine;
+      }
+      for (; i < n; ++i) rank += list[i] > mine;
+      if (rank < k) emit(rank, mine);
+    }
+    return;
   }
+  int size = 256;
+  while (size < n) size *= 2;
+  for (int j = n + threadIdx.x; j < size; j += NT) list[j] = 0;
+  __syncthreads();
+  for (int run = 2; run <= size; run *= 2)
+    for (int apart = run / 2; apart > 0; apart /= 2) {
+      for (int t = threadIdx.x; t < size / 2; t += NT) {
+        const int i = (t & ~(apart - 1)) << 1 | (t & (apart - 1)), j = i + apart;
+        const uint64_t x = list[i], y = list[j];
+        if ((x < y) == ((i & run) == 0)) {
+          list[i] = y;
+          list[j] = x;
+        }
+      }
+      __syncthreads();
+    }
+  for (int j = threadIdx.x; j < n && j < k; j += NT) emit(j, list[j]);
 }
 
 // emit(rank, entry) for the first `need` columns of the range whose logit is of this order, from `rank` on; returns how many
@@ -298,29 +414,55 @@ __device__ void pick_by_digits(PickLds<NT>& lds, uint64_t* list, const typename 
   rank_equal<D, NT>(lds, row, begin, end, order, need, kk - need, emit);
 }
 
-// emit(rank, entry) once for every rank below k that the range has, by any thread.  `groups`: the maxima that the walk left in
-// LDS, at least kCandidates entries long; they are overwritten.  meet() has run.
-template <class D, bool VEC, int NT, class Emit>
-__device__ __forceinline__ void pick(PickLds<NT>& lds, float* groups, const typename D::type* __restrict__ row, int64_t begin,
-                                     int64_t end, int span, int k, float best, Emit&& emit) {
-  constexpr int G = D::kVec;
-  const int64_t trip = (int64_t)NT * G * kInFlight;
-  const int trips = (int)((end - begin + trip - 1) / trip), slots = (trips + span - 1) / span * NT;
+// Where the logits of a group lie that the walk has left a maximum of: kPieces() x 16 bytes.
+template <class D, int NT>
+struct WalkLayout {
+  using Word = GroupWord<D>;
+  int64_t begin;
+  int words, span;
+  __device__ __forceinline__ int pieces() const { return Word::kLoads * span; }
+  __device__ __forceinline__ int64_t column(int group, int piece) const {
+    const int slot = group / Word::kHalves;
+    const int64_t load = (int64_t)(slot / NT * span + piece / Word::kLoads) * kInFlight + group % Word::kHalves * Word::kLoads + piece % Word::kLoads;
+    return begin + (load * NT + slot % NT) * D::kVec;
+  }
+};
+// Of a tile of the head's epilogue (HeadPickArgs).
+struct TileLayout {
+  using Word = GroupWord<F32>;
+  int words;
+  __device__ __forceinline__ int pieces() const { return 8; }
+  __device__ __forceinline__ int64_t column(int group, int piece) const {
+    return 256 * (int64_t)(group >> 3) + 128 * (group >> 2 & 1) + 4 * (group & 3) + 16 * piece;
+  }
+};
+
+// emit(rank, entry) once for every rank below k that the range has, by any thread.  `groups`: the maxima in LDS, which has room for
+// kCandidates entries; they are overwritten.  meet() has run.
+template <class D, bool VEC, int NT, class Layout, class Emit>
+__device__ __forceinline__ void pick(PickLds<NT>& lds, unsigned* groups, const Layout& layout,
+                                     const typename D::type* __restrict__ row, int64_t begin, int64_t end, int k, float best,
+                                     Emit&& emit) {
+  using Word = typename Layout::Word;
+  constexpr int G = D::kVec, H = Word::kHalves;
   const float least = logit_of(lds.least);
   const bool all_finite = lds.least == kOrderOfMinusInf + 1;
   if (best >= least)
-    for (int slot = threadIdx.x; slot < slots; slot += NT)
-      if (groups[slot] >= least) {
-        const int at = atomicAdd(&lds.groups, 1);
-        if (at < kGroupList) lds.group[at] = slot;
-      }
+    for (int slot = threadIdx.x; slot < layout.words; slot += NT) {
+      const unsigned word = groups[slot];
+#pragma unroll
+      for (int i = 0; i < H; ++i)
+        if (Word::half(word, i) >= least) {
+          const int at = atomicAdd(&lds.groups, 1);
+          if (at < kGroupList) lds.group[at] = slot * H + i;
+        }
+    }
   __syncthreads();
   uint64_t* const list = reinterpret_cast<uint64_t*>(groups);
-  const int pieces = kInFlight * span, n_groups = lds.groups;
+  const int pieces = layout.pieces(), n_groups = lds.groups;
   if (n_groups <= kGroupList) {
     for (int j = threadIdx.x; j < n_groups * pieces; j += NT) {
-      const int slot = lds.group[j / pieces];
-      const int64_t c = begin + ((int64_t)(slot / NT * pieces + j % pieces) * NT + slot % NT) * G;
+      const int64_t c = layout.column(lds.group[j / pieces], j % pieces);
       float x[G];
       if (c + G <= end) {
         const Pack<D> p = __builtin_bit_cast(Pack<D>, load_whole<D, VEC, false>(row + c));
@@ -338,9 +480,9 @@ __device__ __forceinline__ void pick(PickLds<NT>& lds, float* groups, const type
     }
     __syncthreads();
     const int n = lds.candidates;
-    if (n <= kCandidates) {
+    if (n <= kCandidates && (n >= k || all_finite)) {
       rank_list<NT>(list, n, k, emit);
-      if (n < k && all_finite) {
+      if (n < k) {
         // the others are -inf, and then NaN, in the order of their columns
         const int64_t more = end - begin - n;
         const int need = (int)(more < k - n ? more : k - n);
@@ -394,7 +536,7 @@ struct RowResult {
 template <class D, bool VEC, int NT>
 __global__ __launch_bounds__(NT) void row_topk_kernel(TopkArgs a) {
   using T = typename D::type;
-  extern __shared__ __attribute__((aligned(16))) float groups[];
+  extern __shared__ __attribute__((aligned(16))) unsigned groups[];
   __shared__ PickLds<NT> lds;
   const int64_t r = a.splits > 1 ? blockIdx.x / a.splits : blockIdx.x;
   const int split = a.splits > 1 ? (int)(blockIdx.x % a.splits) : 0;
@@ -406,56 +548,90 @@ __global__ __launch_bounds__(NT) void row_topk_kernel(TopkArgs a) {
   else walk<D, VEC, true, NT, true, true>(row, begin, end, a.scale2, a.span, st, best, groups);
   meet<D, NT>(lds, st, best, a.k);
   st = lds.whole;
+  constexpr int64_t trip = (int64_t)NT * D::kVec * kInFlight;
+  const int trips = (int)((end - begin + trip - 1) / trip);
+  const WalkLayout<D, NT> layout{begin, (trips + a.span - 1) / a.span * NT, a.span};
   if (a.splits > 1) {
     const int64_t part = r * a.splits + split;
     uint64_t* const out = a.part_entry + part * a.k;
-    pick<D, VEC, NT>(lds, groups, row, begin, end, a.span, a.k, best, [&](int rank, uint64_t entry) { out[rank] = entry; });
+    pick<D, VEC, NT>(lds, groups, layout, row, begin, end, a.k, best, [&](int rank, uint64_t entry) { out[rank] = entry; });
     for (int64_t j = end - begin + threadIdx.x; j < a.k; j += NT) out[j] = 0;
     if (threadIdx.x == 0) a.part_state[part] = make_float4(st.m, st.s, st.sz, 0.f);
   } else {
     const RowResult result{a, r, st};
-    pick<D, VEC, NT>(lds, groups, row, begin, end, a.span, a.k, best, result);
+    pick<D, VEC, NT>(lds, groups, layout, row, begin, end, a.k, best, result);
     if (threadIdx.x == 0) result.template scalars<D>(row);
   }
 }
 
-// A row's splits: an entry's rank is its place in its own list plus how many of the other lists' are larger.
+// The k largest of a token's logits that the head has written out.
+template <int NT>
+__global__ __launch_bounds__(NT) void head_pick_kernel(HeadPickArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned groups[];
+  __shared__ PickLds<NT> lds;
+  const int64_t tok = blockIdx.x;
+  const float* __restrict__ row = a.z + tok * a.z_ld;
+  const float* __restrict__ maxima = a.group_max + tok * a.groups;
+  float best = -kInf;
+  for (int j = threadIdx.x; j < a.groups; j += NT) {
+    const float x = maxima[j];
+    groups[j] = __float_as_uint(x);
+    best = fmaxf(best, x);
+  }
+  meet<F32, NT>(lds, Softmax{kNegBig, 0.f, 0.f}, best, a.k);
+  const float lse = a.lse[tok];
+  pick<F32, true, NT>(lds, groups, TileLayout{a.groups}, row, 0, a.vocab, a.k, best, [&](int rank, uint64_t entry) {
+    a.top[tok * a.k + rank] = fmaf(logit_of(order_in(entry)), a.rcp_t, -lse);
+    a.index[tok * a.k + rank] = column_in(entry);
+  });
+}
+
+// A row's splits: of S lists that fall, the smallest of their ceil(k / S)-th entries is a value that at least k entries reach, and so is
+// any list's k-th; the entries that reach the larger of the two, usually a few times k, are ranked by counting.
 template <class D>
 __global__ __launch_bounds__(kNarrow) void row_topk_join_kernel(TopkArgs a) {
-  extern __shared__ __attribute__((aligned(16))) float groups[];
+  extern __shared__ __attribute__((aligned(16))) unsigned groups[];
   uint64_t* const list = reinterpret_cast<uint64_t*>(groups);
   __shared__ Softmax whole;
+  __shared__ uint64_t reach;
+  __shared__ int found;
   const int64_t r = blockIdx.x;
-  const int n = a.splits * a.k;
-  for (int j = threadIdx.x; j < n; j += kNarrow) list[j] = a.part_entry[r * n + j];
-  if (threadIdx.x < 64) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = a.splits * a.k, place = (a.k + a.splits - 1) / a.splits - 1;
+  const uint64_t* const parts = a.part_entry + r * n;
+  if (threadIdx.x == 0) found = 0;
+  if (w == 0) {
     Softmax st{kNegBig, 0.f, 0.f};
-    for (int j = threadIdx.x; j < a.splits; j += 64) {
+    for (int j = lane; j < a.splits; j += 64) {
       const float4 x = a.part_state[r * a.splits + j];
       merge(st, Softmax{x.x, x.y, x.z});
     }
     merge_wave(st);
-    if (threadIdx.x == 0) whole = st;
+    if (lane == 0) whole = st;
+  } else if (w == 1) {
+    uint64_t least = ~0ull, last = 0;
+    for (int j = lane; j < a.splits; j += 64) {
+      const uint64_t x = parts[j * a.k + place], y = parts[j * a.k + a.k - 1];
+      least = x < least ? x : least;
+      last = y > last ? y : last;
+    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) {
+      const uint64_t x = __shfl_xor(least, off, 64), y = __shfl_xor(last, off, 64);
+      least = x < least ? x : least;
+      last = y > last ? y : last;
+    }
+    least = last > least ? last : least;
+    if (lane == 0) reach = least > 0 ? least : 1;  // (0: no entry)
+  }
+  __syncthreads();
+  const uint64_t least = reach;
+  for (int j = threadIdx.x; j < n; j += kNarrow) {
+    const uint64_t x = parts[j];
+    if (x >= least) list[atomicAdd(&found, 1)] = x;
   }
   __syncthreads();
   const RowResult result{a, r, whole};
-  for (int j = threadIdx.x; j < n; j += kNarrow) {
-    const uint64_t mine = list[j];
-    if (mine == 0) continue;
-    const int own = j / a.k;
-    int rank = j - own * a.k;
-    for (int other = 0; other < a.splits && rank < a.k; ++other) {
-      if (other == own) continue;
-      int lo = 0, hi = a.k;  // how many of a list that falls are larger
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (list[other * a.k + mid] > mine) lo = mid + 1;
-        else hi = mid;
-      }
-      rank += lo;
-    }
-    if (rank < a.k) result(rank, mine);
-  }
+  rank_list<kNarrow>(list, found, a.k, result);
   if (threadIdx.x == 0) result.template scalars<D>(static_cast<const typename D::type*>(a.logits) + r * a.ld);
 }
 
@@ -639,16 +815,17 @@ __global__ __launch_bounds__(kNarrow) void row_topk_weight_kernel(const float* d
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------
-// Up to 64 alternatives the maxima of 256 threads give a value that about k logits reach; for more, 1024 threads.
-int threads_for(int k) { return k <= 64 ? kNarrow : kWide; }
+// The maxima of how many threads give the value that about k logits reach.  4096 x 152064 bf16, 256, 512 and 1024 threads, us:
+// k = 65 228, 242 and 325, 128 257, 265 and 341, 160 286, 272 and 350, 256 (256 threads: every maximum is reached) 326 and 434.
+int threads_for(int k) { return k <= 128 ? kNarrow : kMiddle; }
 
-constexpr int kJoinEntries = 6144;  // 48 KB of LDS in row_topk_join_kernel
+constexpr int kJoinEntries = 4096;  // 32 KB of LDS in row_topk_join_kernel; a power of two, which rank_list may need
 
 struct TopkPlan {
   int threads, span, splits;
   int64_t split_cols, slots;  // slots: group maxima per workgroup
   size_t lds_bytes() const {
-    const size_t list = kCandidates * sizeof(uint64_t), maxima = (size_t)slots * sizeof(float);
+    const size_t list = kCandidates * sizeof(uint64_t), maxima = (size_t)slots * sizeof(unsigned);
     return maxima > list ? maxima : list;
   }
 };
@@ -657,17 +834,19 @@ TopkPlan plan_topk(int64_t n_rows, int64_t vocab, int dtype, int k) {
   p.threads = threads_for(k);
   const int64_t trip = (int64_t)p.threads * (dtype == VAMD_DT_F32 ? 4 : 8) * kInFlight;
   int64_t trips = (vocab + trip - 1) / trip;
-  // Few rows: a row is shared out over workgroups, a trip or more each, until there are four to a CU.
-  const int64_t workgroups = (int64_t)device_cu_count() * (4 * kNarrow / p.threads);
+  // Few rows: a row is shared out over workgroups, at least a trip each, until there are two of 256 threads to a CU (two, three,
+  // four and eight, us: 64 x 152064 bf16 k = 20 16.2, 16.6, 21.5 and 22.2, 200 rows 23.4, 23.4, 23.2 and 27.2, 32 rows 15.1, 17.0,
+  // 17.1 and 16.9).
+  const int64_t workgroups = (int64_t)device_cu_count() * 2 * kNarrow / p.threads;
   int64_t splits = n_rows < 2 * device_cu_count() ? workgroups / n_rows : 1;
   if (splits > trips) splits = trips;
   if (splits > kJoinEntries / k) splits = kJoinEntries / k;
   if (splits < 1) splits = 1;
-  const int64_t each = (trips + splits - 1) / splits;
-  p.splits = (int)((trips + each - 1) / each);
-  p.split_cols = p.splits > 1 ? each * trip : vocab;
-  trips = p.splits > 1 ? each : trips;
-  const int64_t most = kGroupBytes / (int64_t)sizeof(float) / p.threads;  // groups per thread
+  // equal parts, so that each part's list is as deep into the row's alternatives as the others
+  p.split_cols = splits > 1 ? ((vocab + splits - 1) / splits + 7) / 8 * 8 : vocab;
+  p.splits = (int)((vocab + p.split_cols - 1) / p.split_cols);
+  trips = (p.split_cols + trip - 1) / trip;
+  const int64_t most = kGroupBytes / (int64_t)sizeof(unsigned) / p.threads;  // words per thread
   p.span = (int)((trips + most - 1) / most);
   p.slots = (trips + p.span - 1) / p.span * p.threads;
   return p;
@@ -728,6 +907,17 @@ int entries_backward(EntriesArgs a, int dtype, int64_t n_rows, hipStream_t s) {
 }
 
 }  // namespace
+
+int launch_head_pick(const HeadPickArgs& a, hipStream_t s) {
+  const size_t list = kCandidates * sizeof(uint64_t), maxima = (size_t)a.groups * sizeof(float);
+  if (threads_for(a.k) == kNarrow)
+    hipLaunchKernelGGL((head_pick_kernel<kNarrow>), dim3((unsigned)a.n_tokens), dim3(kNarrow), maxima > list ? maxima : list, s, a);
+  else
+    hipLaunchKernelGGL((head_pick_kernel<kMiddle>), dim3((unsigned)a.n_tokens), dim3(kMiddle), maxima > list ? maxima : list, s, a);
+  VAMD_LAUNCH_CHECK();
+  return VAMD_OK;
+}
+
 }  // namespace vamd
 
 using namespace vamd;
@@ -768,12 +958,12 @@ extern "C" int vamd_row_topk(const void* logits, int dtype, int64_t n_rows, int6
     a.cached_rows = cached_rows(n_rows, ld, sizeof(typename D::type));
     const bool vec = rows_vectorizable<D>(logits, ld);
     const auto launch = p.threads == kNarrow ? (vec ? launch_topk<D, true, kNarrow> : launch_topk<D, false, kNarrow>)
-                                             : (vec ? launch_topk<D, true, kWide> : launch_topk<D, false, kWide>);
+                                             : (vec ? launch_topk<D, true, kMiddle> : launch_topk<D, false, kMiddle>);
     launch(a, n_rows * p.splits, p.lds_bytes(), s);
     if (p.splits > 1) {
       VAMD_LAUNCH_CHECK();
       hipLaunchKernelGGL((row_topk_join_kernel<D>), dim3((unsigned)n_rows), dim3(kNarrow),
-                         (size_t)p.splits * k * sizeof(uint64_t), s, a);
+                         kJoinEntries * sizeof(uint64_t), s, a);
     }
   });
   VAMD_LAUNCH_CHECK();

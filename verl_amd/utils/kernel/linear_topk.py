@@ -11,8 +11,7 @@ import torch
 
 from ... import _cabi
 from ..torch_functional import divergence_code
-from .linear_cross_entropy import (_check_inputs, _new_logits_cache, active_token_index, efficient_entropy_forward,
-                                   keeps_logits)
+from .linear_cross_entropy import _check_inputs, _new_logits_cache, active_token_index, keeps_logits
 
 TOPK_MAX = 256   # VAMD_TOPK_MAX
 
@@ -100,13 +99,18 @@ class LinearTopkDistillation(torch.autograd.Function):
         follows = grad_mode and (ctx.needs_input_grad[0] or ctx.needs_input_grad[1])
         cache = _new_logits_cache(n, v, dev) if follows and keeps_logits(n, v, dev) else None
         no_labels = torch.full((n,), -1, dtype=torch.int64, device=dev)
-        _, _, lse, _ = efficient_entropy_forward(hidden, weight, no_labels, 0, temperature, logits_cache=cache)
-        loss = torch.empty(n, dtype=torch.float32, device=dev)
+        _check_inputs(hidden, weight, no_labels)
+        lse, scratch, loss = (torch.empty(s, dtype=torch.float32, device=dev) for s in (n, 3 * n, n))
         slope_sum, slope, prob = (torch.empty(s, dtype=torch.float32, device=dev) if follows else None
                                   for s in ((n,), (n, k), (n, k)))
-        with _cabi.device_guard(dev):
-            _cabi.check(_cabi.lib().vamd_lce_divergence(
-                hidden.data_ptr(), weight.data_ptr(), _cabi.ptr(cache), n, hidden.shape[1], v, t.data_ptr(), index.data_ptr(), k,
+        L, h = _cabi.lib(), hidden.shape[1]
+        with _cabi.device_guard(dev):   # the query as well: it counts the current device's compute units
+            ws = _cabi.workspace(L.vamd_lce_forward_workspace_bytes(n, h, v), dev)
+            _cabi.check(L.vamd_lce_divergence_forward(
+                hidden.data_ptr(), weight.data_ptr(), no_labels.data_ptr(), n, h, v, 1.0 / temperature, scratch.data_ptr(),
+                lse.data_ptr(), _cabi.ptr(cache), ws.data_ptr(), ws.numel(), _cabi.stream_ptr(dev)))
+            _cabi.check(L.vamd_lce_divergence(
+                hidden.data_ptr(), weight.data_ptr(), _cabi.ptr(cache), n, h, v, t.data_ptr(), index.data_ptr(), k,
                 code, beta, 1.0 / temperature, lse.data_ptr(), loss.data_ptr(), _cabi.ptr(slope_sum), _cabi.ptr(slope),
                 _cabi.ptr(prob), _cabi.stream_ptr(dev)))
         ctx.save_for_backward(hidden, weight, index, lse, slope_sum, slope, prob, cache)
