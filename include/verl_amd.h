@@ -282,8 +282,8 @@ int vamd_row_divergence_backward(const void* logits, int dtype, int64_t n_rows, 
  * labels and results of vamd_lce_forward.
  * vamd_lce_topk: logprobs, entropy, top and index as vamd_row_topk's, of the fp32 products hidden . weight; the logits of
  *   token_chunk tokens at a time (0: a few thousand) lie in the workspace.
- * vamd_lce_divergence_forward: the lse, and the logits cache or NULL, of vamd_lce_forward with the sums of each tile formed
- *   apart; scratch: fp32 [3 * n_tokens]; workspace as vamd_lce_forward's; no_labels: int64 [n_tokens], all -1.
+ * vamd_lce_divergence_forward: the log-sum-exp, as lse + lse_rest, and the logits cache, or NULL, of vamd_lce_forward with the
+ *   sums of each tile formed apart; scratch: fp32 [3 * n_tokens]; workspace as vamd_lce_forward's; no_labels: int64 [n_tokens], all -1.
  * vamd_lce_divergence: the loss, for that lse and logits cache (or NULL);
  *   slope_sum [n_tokens], slope and prob [n_tokens, k] (fp32) are what the backward pass needs, NULL together without one.
  * vamd_lce_divergence_backward: vamd_lce_backward_subset_rows for d_loss [n_tokens] and d_loss_slope = d_loss * slope_sum. */
@@ -293,11 +293,11 @@ int vamd_lce_topk(const void* hidden, const void* weight, const int64_t* labels,
                   int64_t token_chunk, void* workspace, size_t workspace_bytes, void* stream);
 int vamd_lce_divergence_forward(const void* hidden, const void* weight, const int64_t* no_labels, int64_t n_tokens,
                                 int64_t hidden_size, int64_t vocab, float rcp_temperature, float* scratch, float* lse,
-                                float* logits_cache, void* workspace, size_t workspace_bytes, void* stream);
+                                float* lse_rest, float* logits_cache, void* workspace, size_t workspace_bytes, void* stream);
 int vamd_lce_divergence(const void* hidden, const void* weight, const float* logits_cache, int64_t n_tokens,
                         int64_t hidden_size, int64_t vocab, const float* teacher_logprobs, const int64_t* teacher_index, int k,
-                        int divergence, float beta, float rcp_temperature, const float* lse, float* loss, float* slope_sum,
-                        float* slope, float* prob, void* stream);
+                        int divergence, float beta, float rcp_temperature, const float* lse, const float* lse_rest, float* loss,
+                        float* slope_sum, float* slope, float* prob, void* stream);
 int vamd_lce_divergence_backward(const void* hidden, const void* weight, const int64_t* no_labels, int64_t n_tokens,
                                  int64_t planned_tokens, int64_t hidden_size, int64_t vocab, const int64_t* teacher_index,
                                  int k, float rcp_temperature, const float* lse, const float* slope_sum, const float* slope,

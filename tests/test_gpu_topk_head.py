@@ -350,7 +350,7 @@ def test_refusals_on_the_host():
     assert topk(size=need - 1) == -2 and topk(ws=None) == -2
     assert lib.vamd_lce_topk_workspace_bytes(100000, 3584, 152064, 64, 0) < 4 << 30   # a few thousand tokens at a time
     div = lambda hidden=at, cache=None, v=300, teacher=at, k=5, kind=0, beta=0.5, rcp=1.0, slope=at, prob=at: lib.vamd_lce_divergence(
-        hidden, at, cache, 4, 128, v, teacher, at, k, kind, beta, rcp, at, at, at, slope, prob, None)
+        hidden, at, cache, 4, 128, v, teacher, at, k, kind, beta, rcp, at, at, at, at, slope, prob, None)
     for bad in (dict(hidden=None), dict(hidden=at + 8), dict(cache=at, v=300 + 1), dict(teacher=None), dict(k=0), dict(k=257),
                 dict(kind=3), dict(kind=2, beta=0.0), dict(rcp=-1.0), dict(slope=None), dict(prob=None)):
         assert div(**bad) == -1, bad

@@ -83,9 +83,9 @@ SIGNATURES = {
     "vamd_lce_topk": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_float, c_void_p, c_void_p,
                               c_void_p, c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
     "vamd_lce_divergence_forward": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_float, c_void_p,
-                                            c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+                                            c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "vamd_lce_divergence": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int,
-                                    c_float, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+                                    c_float, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "vamd_lce_divergence_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int,
                                              c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                              c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_size_t,

@@ -837,6 +837,9 @@ struct MergeArgs {
   float* lse;
   float* mean_z;
   float* sum_pi_squared;
+  // or null: what the log-sum-exp lacks as an fp32 number.  A log-prob near 0 is the difference of two numbers near 30.
+  float* lse_rest;
+  double scale_error;  // of scale2 against log2(e) rcp_t, relative: the sums' temperature is off by that from the logits'
 };
 
 // Combines the partial states of a token.  `1 << lanes_log2` consecutive lanes share a token: each walks every
@@ -887,10 +890,16 @@ __global__ __launch_bounds__(256) void lce_merge_kernel(MergeArgs a) {
   if (a.pi2_partials) a.sum_pi_squared[tok] = q / (s * s);
   const float lse = (m + log2f(s)) * kLn2;
   const float mz = (sy / s) * a.rcp_t;
-  a.lse[tok] = lse;
   a.mean_z[tok] = mz;
   a.entropy[tok] = lse - mz;
   a.logprobs[tok] = zl - lse;
+  if (a.lse_rest) {
+    const double exact = ((double)m + log2((double)s)) * 0.6931471805599453 - a.scale_error * mz;
+    a.lse[tok] = (float)exact;
+    a.lse_rest[tok] = (float)(exact - (float)exact);
+  } else {
+    a.lse[tok] = lse;
+  }
 }
 
 // =============================================================================================
@@ -1207,7 +1216,8 @@ struct HeadDivergenceArgs {
   const uint16_t* hidden;
   const uint16_t* weight;
   const float* z_cache;  // [n_tokens][vocab] logits / temperature, or null
-  const float* lse;
+  const float* lse;      // the log-sum-exp is the sum of the two
+  const float* lse_rest;
   const float* teacher;  // [n_tokens][k] log-probabilities
   const int64_t* index;  // [n_tokens][k]
   int64_t vocab;
@@ -1254,7 +1264,7 @@ __global__ __launch_bounds__(256) void lce_divergence_kernel(HeadDivergenceArgs 
   if (e < a.k) {
     float q = -1.f;
     if (counts(e)) {
-      const float log_q = z[e] - a.lse[tok];
+      const float log_q = (z[e] - a.lse[tok]) - a.lse_rest[tok];
       mine = divergence_term(a.kind, a.beta, teacher[e], log_q);
       q = expf(log_q);
     }
@@ -1849,13 +1859,13 @@ extern "C" size_t vamd_lce_forward_workspace_bytes(int64_t n_tokens, int64_t hid
   return (size_t)plan_forward(n_tokens, vocab).slots() * kTile * (sizeof(float4) + sizeof(float));  // state + squared sums
 }
 
-// Forward launches shared by the two entry points; `workspace` holds at least
-// vamd_lce_forward_workspace_bytes() bytes and the arguments have been checked.
+// Forward launches shared by the entry points; `workspace` holds at least
+// vamd_lce_forward_workspace_bytes() bytes and the arguments have been checked.  Without logprobs the partial states are left as they are.
 static int lce_forward_launch(const void* hidden, const void* weight, const int64_t* labels, int64_t n_tokens,
                               int64_t hidden_size, int64_t vocab, float rcp_temperature, float* logprobs,
                               float* entropy, float* lse, float* mean_z, float* logits_cache, float* sum_pi_squared,
                               void* workspace, void* stream, int64_t max_slots = INT64_MAX, Purpose why = kLogprobs,
-                              int64_t z_ld = 0, float z_scale = 0.f, float* group_max = nullptr) {
+                              int64_t z_ld = 0, float z_scale = 0.f, float* group_max = nullptr, float* lse_rest = nullptr) {
   FwdArgs a;
   a.hidden = Operand{static_cast<const uint16_t*>(hidden), hidden_size, (int)n_tokens, (int)hidden_size};
   a.weight = Operand{static_cast<const uint16_t*>(weight), hidden_size, (int)vocab, (int)hidden_size};
@@ -1889,6 +1899,7 @@ static int lce_forward_launch(const void* hidden, const void* weight, const int6
     hipLaunchKernelGGL(kernel, grid, block, lds_bytes, s, a);
   }
   VAMD_LAUNCH_CHECK();
+  if (!logprobs) return VAMD_OK;
 
   MergeArgs m;
   m.partials = a.partials;
@@ -1905,6 +1916,8 @@ static int lce_forward_launch(const void* hidden, const void* weight, const int6
   m.entropy = entropy;
   m.lse = lse;
   m.mean_z = mean_z;
+  m.lse_rest = lse_rest;
+  m.scale_error = (double)a.scale2 / (1.4426950408889634 * (double)rcp_temperature) - 1.0;
   {
     ScopedTiming tm(kTagMerge, s);
     hipLaunchKernelGGL(lce_merge_kernel, dim3((unsigned)ceil_div(n_tokens << m.lanes_log2, 256)), dim3(256), 0, s, m);
@@ -2275,13 +2288,15 @@ extern "C" int vamd_lce_backward_subset_rows(const void* hidden, const void* wei
 // Divergence from a teacher's tokens
 extern "C" int vamd_lce_divergence_forward(const void* hidden, const void* weight, const int64_t* no_labels, int64_t n_tokens,
                                            int64_t hidden_size, int64_t vocab, float rcp_temperature, float* scratch, float* lse,
-                                           float* logits_cache, void* workspace, size_t workspace_bytes, void* stream) {
+                                           float* lse_rest, float* logits_cache, void* workspace, size_t workspace_bytes,
+                                           void* stream) {
   float* const logprobs = scratch;
   float* const entropy = scratch ? scratch + n_tokens : nullptr;
   float* const mean_z = scratch ? scratch + 2 * n_tokens : nullptr;
   int st = check_forward_args(hidden, weight, no_labels, n_tokens, hidden_size, vocab, rcp_temperature, logprobs, entropy, lse,
                               mean_z, logits_cache);
   if (st != VAMD_OK) return st;
+  VAMD_REQUIRE(lse_rest, "lce_divergence_forward: null pointer");
   const size_t need = vamd_lce_forward_workspace_bytes(n_tokens, hidden_size, vocab);
   if (!workspace || workspace_bytes < need) {
     set_error("lce_divergence_forward: workspace %zu bytes, need %zu", workspace_bytes, need);
@@ -2289,24 +2304,25 @@ extern "C" int vamd_lce_divergence_forward(const void* hidden, const void* weigh
   }
   if ((st = ensure_lds_attributes()) != VAMD_OK) return st;
   return lce_forward_launch(hidden, weight, no_labels, n_tokens, hidden_size, vocab, rcp_temperature, logprobs, entropy, lse,
-                            mean_z, logits_cache, nullptr, workspace, stream, INT64_MAX, kDivergence);
+                            mean_z, logits_cache, nullptr, workspace, stream, INT64_MAX, kDivergence, 0, 0.f, nullptr, lse_rest);
 }
 
 extern "C" int vamd_lce_divergence(const void* hidden, const void* weight, const float* logits_cache, int64_t n_tokens,
                                    int64_t hidden_size, int64_t vocab, const float* teacher_logprobs,
                                    const int64_t* teacher_index, int k, int divergence, float beta, float rcp_temperature,
-                                   const float* lse, float* loss, float* slope_sum, float* slope, float* prob, void* stream) {
+                                   const float* lse, const float* lse_rest, float* loss, float* slope_sum, float* slope,
+                                   float* prob, void* stream) {
   int st = check_head_shapes(n_tokens, hidden_size, vocab, logits_cache);
   if (st != VAMD_OK) return st;
   if ((st = check_divergence("lce_divergence", k, divergence, beta)) != VAMD_OK) return st;
-  VAMD_REQUIRE(hidden && weight && teacher_logprobs && teacher_index && lse && loss, "lce_divergence: null pointer");
+  VAMD_REQUIRE(hidden && weight && teacher_logprobs && teacher_index && lse && lse_rest && loss, "lce_divergence: null pointer");
   VAMD_REQUIRE((slope_sum && slope && prob) || !(slope_sum || slope || prob),
                "lce_divergence: slope_sum, slope and prob are written together or not at all");
   VAMD_REQUIRE((reinterpret_cast<uintptr_t>(hidden) | reinterpret_cast<uintptr_t>(weight)) % 16 == 0,
                "lce_divergence: hidden and weight must be 16-byte aligned");
   VAMD_REQUIRE(rcp_temperature > 0.f, "lce_divergence: temperature must be positive");
   const HeadDivergenceArgs a{static_cast<const uint16_t*>(hidden), static_cast<const uint16_t*>(weight), logits_cache, lse,
-                             teacher_logprobs, teacher_index, vocab, (int)n_tokens, (int)hidden_size, k, divergence, beta,
+                             lse_rest, teacher_logprobs, teacher_index, vocab, (int)n_tokens, (int)hidden_size, k, divergence, beta,
                              rcp_temperature, loss, slope_sum, slope, prob};
   hipLaunchKernelGGL(lce_divergence_kernel, dim3((unsigned)n_tokens), dim3(256), 0, static_cast<hipStream_t>(stream), a);
   VAMD_LAUNCH_CHECK();
@@ -2349,7 +2365,7 @@ static int64_t topk_tokens(int64_t n_tokens, int64_t requested) {
   return each < n_tokens ? each : n_tokens;
 }
 
-// Over few tokens, or a vocabulary whose group maxima do not fit into LDS, the rows are read again.
+// Over few tokens, or a vocabulary whose group maxima do not fit into LDS, the rows are read again, and everything comes from them.
 static bool topk_from_groups(int64_t n_tokens, int64_t vocab) {
   return n_tokens > kFewTokens && ceil_div(vocab, kTile) * 8 <= kHeadPickGroups;
 }
@@ -2393,16 +2409,16 @@ extern "C" int vamd_lce_topk(const void* hidden, const void* weight, const int64
     const bool groups = topk_from_groups(n, vocab);
     float* const group_max = groups ? carve.take<float>((size_t)n * ceil_div(vocab, kTile) * 8) : nullptr;
     st = lce_forward_launch(static_cast<const uint16_t*>(hidden) + t0 * hidden_size, weight, labels + t0, n, hidden_size, vocab,
-                            rcp_temperature, logprobs + t0, entropy + t0, lse, lse + n, z, nullptr, forward, stream, INT64_MAX,
-                            groups ? kAlternatives : kDivergence, pitch, 1.f, group_max);
+                            rcp_temperature, groups ? logprobs + t0 : nullptr, entropy + t0, lse, lse + n, z, nullptr, forward, stream,
+                            INT64_MAX, groups ? kAlternatives : kDivergence, pitch, 1.f, group_max);
     if (st != VAMD_OK) return st;
     if (groups) {
       st = launch_head_pick(HeadPickArgs{z, pitch, vocab, group_max, (int)(ceil_div(vocab, kTile) * 8), lse, (int)n, k,
                                          rcp_temperature, top + t0 * k, index + t0 * k}, static_cast<hipStream_t>(stream));
     } else {
       const size_t row_bytes = vamd_row_topk_workspace_bytes(n, vocab, VAMD_DT_F32, k);
-      st = vamd_row_topk(z, VAMD_DT_F32, n, vocab, pitch, nullptr, k, rcp_temperature, nullptr, nullptr, top + t0 * k,
-                         index + t0 * k, nullptr, carve.take<char>(row_bytes), row_bytes, stream);
+      st = vamd_row_topk(z, VAMD_DT_F32, n, vocab, pitch, labels + t0, k, rcp_temperature, logprobs + t0, entropy + t0,
+                         top + t0 * k, index + t0 * k, nullptr, carve.take<char>(row_bytes), row_bytes, stream);
     }
     if (st != VAMD_OK) return st;
   }

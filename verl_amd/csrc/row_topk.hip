@@ -838,7 +838,7 @@ TopkPlan plan_topk(int64_t n_rows, int64_t vocab, int dtype, int k) {
   // four and eight, us: 64 x 152064 bf16 k = 20 16.2, 16.6, 21.5 and 22.2, 200 rows 23.4, 23.4, 23.2 and 27.2, 32 rows 15.1, 17.0,
   // 17.1 and 16.9).
   const int64_t workgroups = (int64_t)device_cu_count() * 2 * kNarrow / p.threads;
-  int64_t splits = n_rows < 2 * device_cu_count() ? workgroups / n_rows : 1;
+  int64_t splits = workgroups / n_rows;
   if (splits > trips) splits = trips;
   if (splits > kJoinEntries / k) splits = kJoinEntries / k;
   if (splits < 1) splits = 1;

@@ -14,6 +14,7 @@ from ..torch_functional import divergence_code
 from .linear_cross_entropy import _check_inputs, _new_logits_cache, active_token_index, keeps_logits
 
 TOPK_MAX = 256   # VAMD_TOPK_MAX
+FEW_TOKENS = 128   # up to which the head's kernels are bound by reading the weight
 
 
 def _check_temperature(temperature: float) -> None:
@@ -60,7 +61,7 @@ def linear_topk_logprobs(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
     return (None if labels is None else logprobs.view(lead), entropy.view(lead), top.view(*lead, k), index.view(*lead, k))
 
 
-def _backward(d_loss, hidden, weight, index, lse, slope_sum, slope, prob, temperature, need_dh, need_dw, cache,
+def _backward(d_loss, hidden, weight, no_labels, index, lse, slope_sum, slope, prob, temperature, need_dh, need_dw, cache,
               planned=None, rows=None):
     """Both gradients over the tokens given; ``rows`` and ``planned`` as in ``efficient_entropy_backward``."""
     n, h = hidden.shape
@@ -69,7 +70,6 @@ def _backward(d_loss, hidden, weight, index, lse, slope_sum, slope, prob, temper
     planned = n if planned is None else planned
     d_hidden = torch.empty_like(hidden) if need_dh else None
     d_weight = torch.empty_like(weight) if need_dw else None
-    no_labels = torch.full((n,), -1, dtype=torch.int64, device=dev)
     d_slope = d_loss * slope_sum
     L = _cabi.lib()
     with _cabi.device_guard(dev):
@@ -100,7 +100,7 @@ class LinearTopkDistillation(torch.autograd.Function):
         cache = _new_logits_cache(n, v, dev) if follows and keeps_logits(n, v, dev) else None
         no_labels = torch.full((n,), -1, dtype=torch.int64, device=dev)
         _check_inputs(hidden, weight, no_labels)
-        lse, scratch, loss = (torch.empty(s, dtype=torch.float32, device=dev) for s in (n, 3 * n, n))
+        lse, rest, scratch, loss = (torch.empty(s, dtype=torch.float32, device=dev) for s in (n, n, 3 * n, n))
         slope_sum, slope, prob = (torch.empty(s, dtype=torch.float32, device=dev) if follows else None
                                   for s in ((n,), (n, k), (n, k)))
         L, h = _cabi.lib(), hidden.shape[1]
@@ -108,12 +108,12 @@ class LinearTopkDistillation(torch.autograd.Function):
             ws = _cabi.workspace(L.vamd_lce_forward_workspace_bytes(n, h, v), dev)
             _cabi.check(L.vamd_lce_divergence_forward(
                 hidden.data_ptr(), weight.data_ptr(), no_labels.data_ptr(), n, h, v, 1.0 / temperature, scratch.data_ptr(),
-                lse.data_ptr(), _cabi.ptr(cache), ws.data_ptr(), ws.numel(), _cabi.stream_ptr(dev)))
+                lse.data_ptr(), rest.data_ptr(), _cabi.ptr(cache), ws.data_ptr(), ws.numel(), _cabi.stream_ptr(dev)))
             _cabi.check(L.vamd_lce_divergence(
                 hidden.data_ptr(), weight.data_ptr(), _cabi.ptr(cache), n, h, v, t.data_ptr(), index.data_ptr(), k,
-                code, beta, 1.0 / temperature, lse.data_ptr(), loss.data_ptr(), _cabi.ptr(slope_sum), _cabi.ptr(slope),
+                code, beta, 1.0 / temperature, lse.data_ptr(), rest.data_ptr(), loss.data_ptr(), _cabi.ptr(slope_sum), _cabi.ptr(slope),
                 _cabi.ptr(prob), _cabi.stream_ptr(dev)))
-        ctx.save_for_backward(hidden, weight, index, lse, slope_sum, slope, prob, cache)
+        ctx.save_for_backward(hidden, weight, no_labels, index, lse, slope_sum, slope, prob, cache)
         ctx.hidden_shape = shape
         ctx.temperature = temperature
         return loss.view(lead)
@@ -121,16 +121,17 @@ class LinearTopkDistillation(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_loss):
-        hidden, weight, index, lse, slope_sum, slope, prob, cache = ctx.saved_tensors
+        hidden, weight, no_labels, index, lse, slope_sum, slope, prob, cache = ctx.saved_tensors
         need_dh, need_dw = ctx.needs_input_grad[:2]
         if d_loss is None or not (need_dh or need_dw):
             return (None,) * 8
         g = d_loss.reshape(-1).to(torch.float32).contiguous()
-        # tokens that the loss masked out are left out of the kernels, as in linear_cross_entropy
-        idx = active_token_index(g, None, hidden.shape[0], weight.shape)
+        # tokens that the loss masked out are left out of the kernels, as in linear_cross_entropy; not of few, over which they wait
+        # for the weight, however many there are (93 x 896 x 151936, an eighth of them masked out: 360 us with and 247 without)
+        idx = active_token_index(g, None, hidden.shape[0], weight.shape) if hidden.shape[0] > FEW_TOKENS else None
         if idx is None:
-            d_hidden, d_weight = _backward(g, hidden, weight, index, lse, slope_sum, slope, prob, ctx.temperature, need_dh,
-                                           need_dw, cache)
+            d_hidden, d_weight = _backward(g, hidden, weight, no_labels, index, lse, slope_sum, slope, prob, ctx.temperature,
+                                           need_dh, need_dw, cache)
         else:
             d_hidden = torch.zeros_like(hidden) if need_dh else None
             d_weight = None
@@ -138,7 +139,7 @@ class LinearTopkDistillation(torch.autograd.Function):
                 d_weight = torch.zeros_like(weight) if need_dw else None
             else:
                 take = lambda x: x.index_select(0, idx)
-                dh, d_weight = _backward(take(g), take(hidden), weight, take(index), take(lse), take(slope_sum), take(slope),
+                dh, d_weight = _backward(take(g), take(hidden), weight, no_labels[:idx.numel()], take(index), take(lse), take(slope_sum), take(slope),
                                          take(prob), ctx.temperature, need_dh, need_dw, cache, hidden.shape[0],
                                          None if cache is None else idx)
                 if need_dh:
