@@ -256,28 +256,30 @@ size_t vamd_row_topk_workspace_bytes(int64_t n_rows, int64_t vocab, int dtype, i
 int vamd_row_topk(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t ld, const int64_t* labels, int k,
                   float rcp_temperature, float* logprobs, float* entropy, float* top, int64_t* index, float* stats,
                   void* workspace, size_t workspace_bytes, void* stream);
-/* Its gradient for upstream gradients of logprobs, entropy [n_rows] and top [n_rows, k], fp32, each of which may be NULL;
- * row_scratch: fp32 [n_rows].  d_logits has the element type of the logits, row pitch ld_out, and is another buffer. */
+/* Its gradient for upstream gradients of logprobs, entropy [n_rows] and top [n_rows, k], fp32, each of which may be NULL.
+ * d_logits has the element type of the logits, row pitch ld_out, and is another buffer. */
+size_t vamd_row_topk_backward_workspace_bytes(int64_t n_rows, int64_t vocab, int dtype, int k);
 int vamd_row_topk_backward(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t ld, const int64_t* labels,
                            int k, const int64_t* index, float rcp_temperature, const float* stats, const float* d_logprobs,
-                           const float* d_entropy, const float* d_top, float* row_scratch, void* d_logits, int64_t ld_out,
-                           void* stream);
+                           const float* d_entropy, const float* d_top, void* d_logits, int64_t ld_out, void* workspace,
+                           size_t workspace_bytes, void* stream);
 /* Divergence of q = softmax(logits / temperature) from a teacher's k tokens (teacher_index, int64) with log-probs t
  * (teacher_logprobs, fp32), both [n_rows, k], p = exp(t), per row:
  *   VAMD_DIV_FORWARD_KL sum p (t - log q), VAMD_DIV_REVERSE_KL sum q (log q - t), VAMD_DIV_JSD beta sum p (t - log w) +
  *   (1 - beta) sum q (log q - log w) with w = beta p + (1 - beta) q, 0 < beta < 1.
  * An entry whose index lies outside [0, vocab) or whose t is -inf adds nothing; a row of such entries has loss 0 and no gradient.
- * stats (fp32 [n_rows, 4], 16-byte aligned) and slope (fp32 [n_rows, k], d loss / d log q) are what the backward pass needs, and
- * may be NULL without one. */
+ * stats (fp32 [n_rows, 4], 16-byte aligned) and entries (vamd_row_divergence_entries_bytes() bytes, 256-byte aligned: what
+ * d loss / d log q is at each entry) are what the backward pass needs, and are NULL together without one. */
 #define VAMD_DIV_FORWARD_KL 0
 #define VAMD_DIV_REVERSE_KL 1
 #define VAMD_DIV_JSD 2
+size_t vamd_row_divergence_entries_bytes(int64_t n_rows, int64_t vocab, int dtype, int k);
 int vamd_row_divergence(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t ld,
                         const float* teacher_logprobs, const int64_t* teacher_index, int k, int divergence, float beta,
-                        float rcp_temperature, float* loss, float* stats, float* slope, void* stream);
+                        float rcp_temperature, float* loss, float* stats, void* entries, size_t entries_bytes, void* stream);
 int vamd_row_divergence_backward(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t ld,
                                  const int64_t* teacher_index, int k, float rcp_temperature, const float* stats,
-                                 const float* slope, const float* d_loss, void* d_logits, int64_t ld_out, void* stream);
+                                 const void* entries, const float* d_loss, void* d_logits, int64_t ld_out, void* stream);
 /* The same two from the head's hidden states [n_tokens, hidden_size] and weight [vocab, hidden_size] (bf16), with the shapes,
  * labels and results of vamd_lce_forward.
  * vamd_lce_topk: logprobs, entropy, top and index as vamd_row_topk's, of the fp32 products hidden . weight; the logits of

@@ -502,15 +502,20 @@ def test_refusals_on_the_host():
     assert need > 0 and lib.vamd_row_topk_workspace_bytes(4096, 151936, 1, 20) == 0
     assert topk(dtype=1, n=1, v=151936, ld=151936, k=20, size=need - 1) == -2
     assert topk(dtype=1, n=1, v=151936, ld=151936, k=20, ws=None) == -2
-    div = lambda kind=0, beta=0.5, teacher=at, index=at, loss=at, k=5, stats=at: lib.vamd_row_divergence(
-        at, 0, 4, 300, 300, teacher, index, k, kind, beta, 1.0, loss, stats, at, None)
+    div = lambda kind=0, beta=0.5, teacher=at, index=at, loss=at, k=5, stats=at, entries=at, size=1 << 30: lib.vamd_row_divergence(
+        at, 0, 4, 300, 300, teacher, index, k, kind, beta, 1.0, loss, stats, entries, size, None)
     for bad in (dict(kind=3), dict(kind=-1), dict(kind=2, beta=1.0), dict(kind=2, beta=NAN), dict(teacher=None), dict(index=None),
-                dict(loss=None), dict(k=0), dict(k=257), dict(stats=at + 8)):
+                dict(loss=None), dict(k=0), dict(k=257), dict(stats=at + 8), dict(stats=None), dict(entries=None)):
         assert div(**bad) == -1, bad
-    for out, ld in ((None, 300), (at, 300), (at + 1 << 20, 299)):   # no output, the logits themselves, too narrow
-        assert lib.vamd_row_divergence_backward(at, 0, 4, 300, 300, at, 5, 1.0, at, at, at, out, ld, None) == -1
-        assert lib.vamd_row_topk_backward(at, 0, 4, 300, 300, at, 5, at, 1.0, at, at, at, None, at, out, ld, None) == -1
-    other = 1 << 20
-    assert lib.vamd_row_topk_backward(at, 0, 4, 300, 300, at, 5, at, 1.0, at, None, None, None, at, other, 300, None) == -1
-    assert lib.vamd_row_topk_backward(at, 0, 4, 300, 300, None, 5, at, 1.0, at, at, None, None, at, other, 300, None) == -1
-    assert lib.vamd_row_topk_backward(at, 0, 4, 300, 300, at, 5, None, 1.0, at, None, None, at, at, other, 300, None) == -1
+    for k in (5, 65):
+        assert div(k=k, size=lib.vamd_row_divergence_entries_bytes(4, 300, 0, k) - 1) == -2
+    other, need = 1 << 20, lib.vamd_row_topk_backward_workspace_bytes(4, 300, 0, 5)
+    back = lambda labels=at, index=at, stats=at, lp=at, ent=None, top=None, out=other, ld=300, ws=at, size=need: \
+        lib.vamd_row_topk_backward(at, 0, 4, 300, 300, labels, 5, index, 1.0, stats, lp, ent, top, out, ld, ws, size, None)
+    div_back = lambda index=at, k=5, stats=at, entries=at, d_loss=at, out=other, ld=300: lib.vamd_row_divergence_backward(
+        at, 0, 4, 300, 300, index, k, 1.0, stats, entries, d_loss, out, ld, None)
+    for bad in (dict(out=None), dict(out=at), dict(ld=299), dict(stats=None), dict(stats=at + 4)):   # at: the logits themselves
+        assert back(**bad) == -1 and div_back(**bad) == -1, bad
+    assert back(lp=None) == -1 and back(labels=None) == -1 and back(lp=None, top=at, index=None) == -1
+    assert div_back(index=None) == -1 and div_back(entries=None) == -1 and div_back(d_loss=None) == -1 and div_back(k=257) == -1
+    assert back(size=need - 1) == -2 and back(ws=None) == -2

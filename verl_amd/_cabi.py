@@ -73,10 +73,12 @@ SIGNATURES = {
     "vamd_row_topk_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int, c_int]),
     "vamd_row_topk": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int, c_float, c_void_p, c_void_p,
                               c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "vamd_row_topk_backward_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int, c_int]),
     "vamd_row_topk_backward": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int, c_void_p, c_float,
-                                       c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+                                       c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
+    "vamd_row_divergence_entries_bytes": (c_size_t, [c_int64, c_int64, c_int, c_int]),
     "vamd_row_divergence": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int, c_float,
-                                    c_float, c_void_p, c_void_p, c_void_p, c_void_p]),
+                                    c_float, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "vamd_row_divergence_backward": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int, c_float, c_void_p,
                                              c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     "vamd_lce_topk_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int, c_int64]),

@@ -636,6 +636,44 @@ __global__ __launch_bounds__(kNarrow) void row_topk_join_kernel(TopkArgs a) {
 }
 
 // ---- divergence from a teacher's tokens -----------------------------------------------------------------------
+// Entries of a gradient by column, equal columns in their order, those that do not count last; and the first one in each chunk of columns
+// that a workgroup of the backward pass takes.  Where a row has more entries than a wavefront looks through at once.
+struct Sorted {
+  int* column;  // [rows][k]; null: not to be sorted
+  float* grad;  // [rows][k]
+  int* first;   // [rows][chunks + 1]
+  int chunks, chunk_cols;
+};
+constexpr int kUnsortedEntries = 64;
+constexpr int kNoEntry = 0x7fffffff;
+// Thread t < k has entry t.  Every thread comes here.
+template <int NT>
+__device__ __forceinline__ void sort_entries(const Sorted& to, int64_t r, int k, int mine, float grad) {
+  __shared__ int column[kMaxK], sorted[kMaxK];
+  const int t = threadIdx.x;
+  if (t < k) column[t] = mine;
+  __syncthreads();
+  if (t < k) {
+    int rank = 0;
+#pragma unroll 8
+    for (int i = 0; i < k; ++i) rank += column[i] < mine || (column[i] == mine && i < t);
+    sorted[rank] = mine;
+    to.column[r * k + rank] = mine;
+    to.grad[r * k + rank] = grad;
+  }
+  __syncthreads();
+  for (int c = t; c <= to.chunks; c += NT) {
+    const int64_t from = (int64_t)c * to.chunk_cols;
+    int lo = 0, hi = k;
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (sorted[mid] < from) lo = mid + 1;
+      else hi = mid;
+    }
+    to.first[r * (to.chunks + 1) + c] = lo;
+  }
+}
+
 struct DivergenceArgs {
   const void* logits;
   int64_t ld, cols;
@@ -644,8 +682,9 @@ struct DivergenceArgs {
   int k, kind;
   float beta, scale2;
   float* loss;
-  float4* stats;  // m, 1 / s, sum of the slopes, lse
-  float* slope;   // [rows][k]
+  float4* stats;  // m, 1 / s, sum of the slopes, lse; null without a backward pass
+  float* slope;   // [rows][k], where the entries are few
+  Sorted sorted;  // where they are many
   int64_t cached_rows;
 };
 
@@ -681,6 +720,7 @@ __global__ __launch_bounds__(NT) void row_divergence_kernel(DivergenceArgs a) {
   Term mine{0.f, 0.f};
   if (index >= 0) mine = divergence_term(a.kind, a.beta, t, log_q(z, a.scale2, st));
   if (a.slope && (int)threadIdx.x < a.k) a.slope[r * a.k + threadIdx.x] = mine.slope;
+  if (a.sorted.column) sort_entries<NT>(a.sorted, r, a.k, index >= 0 ? (int)index : kNoEntry, mine.slope);
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) {
     mine.loss += __shfl_xor(mine.loss, off, 64);
@@ -714,6 +754,7 @@ struct EntriesArgs {
   int chunks, k;
   const int64_t* index;    // [rows][k]; one outside [0, cols) matches nothing
   const float* grad;       // [rows][k]: g_k
+  Sorted sorted;           // the same where there are more than kUnsortedEntries
   const float4* stats;     // m, 1 / s, ., .
   const float* weight;     // [rows]: sum of all g; null: the third of stats
   const float* scale;      // [rows] or null (1)
@@ -725,15 +766,18 @@ struct EntriesArgs {
   int64_t ld_out;
 };
 
-// One workgroup per (row, chunk of kNarrow * G * F columns), as row_softmax_backward_kernel, whose comments say why.  Every
-// wavefront looks through the row's entries for those of its own columns, 64 at a time, and adds them, in their order, in the
-// registers of the lane that holds the column: an index that comes twice counts twice, and each gradient is rounded once.
-template <class D, bool VEC, bool STREAM>
+// One workgroup per (row, chunk of kNarrow * G * F columns), as row_softmax_backward_kernel, whose comments say why.  An entry is added,
+// in order, in the registers of the lane that holds its column, so that an index that comes twice counts twice and each gradient
+// is rounded once.  Up to 64 entries every wavefront looks through all of the row's for its own: they come with the logits.  More
+// are sorted first, and a workgroup reads its own, behind the place of the first.  4096 x 152064 bf16, forward and backward pass of the
+// divergence, all of them looked through and sorted, us: 5 entries 606 and 605, 64 618 and 632, 128 690 and 649, 256 850 and 683.
+template <class D, bool VEC, bool STREAM, bool SORTED>
 __global__ __launch_bounds__(kNarrow) void row_entries_backward_kernel(EntriesArgs a) {
   using T = typename D::type;
   constexpr int G = D::kVec, F = D::kBackwardLoads;
   const int64_t r = blockIdx.x / a.chunks;
-  const int chunk = blockIdx.x % a.chunks, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int chunk = blockIdx.x % a.chunks, lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const T* __restrict__ row = static_cast<const T*>(a.logits) + r * a.ld;
   T* __restrict__ out = static_cast<T*>(a.out) + r * a.ld_out;
   constexpr int64_t stride = (int64_t)kNarrow * G;
@@ -744,10 +788,24 @@ __global__ __launch_bounds__(kNarrow) void row_entries_backward_kernel(EntriesAr
     const int64_t c = c0 + u * stride;
     if (c + G <= a.cols) raw[u] = load_whole<D, VEC, STREAM>(row + c);
   }
-  const int64_t* const entries = a.index + r * a.k;
-  int64_t entry = lane < a.k ? entries[lane] : -1;
+  const int64_t entries = r * a.k;
+  // the column of the entry that the lane looks at, and its gradient (as they come: a conversion would wait for them here)
+  std::conditional_t<SORTED, int, int64_t> column = -1;
+  float grad = 0.f;
+  if (!SORTED && lane < a.k) column = a.index[entries + lane];
   __builtin_amdgcn_sched_barrier(0);
   const float4 st = a.stats[r];
+  int e_begin = 0, e_end = a.k;
+  if constexpr (SORTED) {
+    const int* const place = a.sorted.first + r * (a.sorted.chunks + 1) + chunk;
+    e_begin = place[0];
+    e_end = place[1];
+    if (e_begin + lane < e_end) {  // requested before the logits are waited for
+      column = a.sorted.column[entries + e_begin + lane];
+      grad = a.sorted.grad[entries + e_begin + lane];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
   const float scale = (a.scale ? a.scale[r] : 1.f) * a.rcp_t;
   const float glp = a.d_logprobs ? a.d_logprobs[r] * a.rcp_t : 0.f;
   const int64_t label = a.d_logprobs ? a.labels[r] : -1;
@@ -774,17 +832,20 @@ __global__ __launch_bounds__(kNarrow) void row_entries_backward_kernel(EntriesAr
       x[u][e] = fmaf(-ex, a.d_entropy ? t : u0, hit == e ? glp : 0.f);
     }
   }
-  for (int e0 = 0; e0 < a.k; e0 += 64) {
-    if (e0 > 0) entry = e0 + lane < a.k ? entries[e0 + lane] : -1;
-    const int64_t rel64 = entry - first;
-    const bool inside = entry < a.cols && rel64 >= 0 && rel64 < stride * F;
+  for (int e0 = e_begin; e0 < e_end; e0 += 64) {
+    if (SORTED && e0 > e_begin && e0 + lane < e_end) {
+      column = a.sorted.column[entries + e0 + lane];
+      grad = a.sorted.grad[entries + e0 + lane];
+    }
+    const int64_t rel64 = (int64_t)column - first;
+    const bool inside = e0 + lane < e_end && column < a.cols && rel64 >= 0 && rel64 < stride * F;
     const int rel = inside ? (int)rel64 : 0;
     uint64_t hits = __ballot(inside && rel / G % kNarrow / 64 == w);
     while (hits) {
       const int b = __ffsll((unsigned long long)hits) - 1;
       hits &= hits - 1;
       const int at = __builtin_amdgcn_readlane(rel, b);
-      const float g = a.grad[r * a.k + e0 + b] * scale;
+      const float g = (SORTED ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(grad), b)) : a.grad[entries + b]) * scale;
       const int mine = at / G % 64 == lane ? at / (int)stride * G + at % G : -1;
 #pragma unroll
       for (int u = 0; u < F; ++u)
@@ -799,20 +860,30 @@ __global__ __launch_bounds__(kNarrow) void row_entries_backward_kernel(EntriesAr
   }
 }
 
-// weight[r] = d_logprobs[r], where the label counts, + sum of d_top[r]; a wavefront per row
-__global__ __launch_bounds__(kNarrow) void row_topk_weight_kernel(const float* d_logprobs, const int64_t* labels, int64_t cols,
-                                                                  const float* d_top, int k, int64_t rows, float* weight) {
-  const int64_t r = (int64_t)blockIdx.x * (kNarrow / 64) + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (r >= rows) return;
-  float sum = 0.f;
-  for (int j = lane; j < k; j += 64) sum += d_top[r * k + j];
+// What the backward pass of the alternatives needs first: weight[r], the sum of d_top[r] and of d_logprobs[r] where the label counts, and
+// where there are many alternatives their order.
+__global__ __launch_bounds__(kNarrow) void row_topk_prepare_kernel(const float* d_logprobs, const int64_t* labels, int64_t cols,
+                                                                   const float* d_top, const int64_t* index, int k, float* weight,
+                                                                   Sorted sorted) {
+  __shared__ float red[kNarrow / 64];
+  const int64_t r = blockIdx.x;
+  const int t = threadIdx.x;
+  const float grad = t < k ? d_top[r * k + t] : 0.f;
+  float sum = grad;
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
-  if (lane != 0) return;
-  if (d_logprobs && labels[r] >= 0 && labels[r] < cols) sum += d_logprobs[r];
-  weight[r] = sum;
+  if ((t & 63) == 0) red[t >> 6] = sum;
+  __syncthreads();
+  if (t == 0) {
+    sum = red[0] + red[1] + red[2] + red[3];
+    if (d_logprobs && labels[r] >= 0 && labels[r] < cols) sum += d_logprobs[r];
+    weight[r] = sum;
+  }
+  if (!sorted.column) return;
+  const int64_t i = t < k ? index[r * k + t] : -1;
+  sort_entries<kNarrow>(sorted, r, k, i >= 0 && i < cols ? (int)i : kNoEntry, grad);
 }
+static_assert(kMaxK <= kNarrow, "an entry per thread");
 
 // ---- host side -------------------------------------------------------------------------------------------------
 // The maxima of how many threads give the value that about k logits reach.  4096 x 152064 bf16, 256, 512 and 1024 threads, us:
@@ -875,10 +946,30 @@ int check_topk(const char* what, const void* logits, int dtype, int64_t n_rows, 
   return VAMD_OK;
 }
 
-template <class D>
-int64_t backward_chunks(int64_t vocab) {
-  const int64_t per_wg = (int64_t)kNarrow * D::kVec * D::kBackwardLoads;
-  return (vocab + per_wg - 1) / per_wg;
+int chunk_columns(int dtype) {
+  return kNarrow * (dtype == VAMD_DT_F32 ? F32::kVec * F32::kBackwardLoads : BF16::kVec * BF16::kBackwardLoads);
+}
+static_assert(BF16::kVec * BF16::kBackwardLoads == F16::kVec * F16::kBackwardLoads, "chunk_columns");
+int64_t chunks_of(int64_t vocab, int dtype) { return (vocab + chunk_columns(dtype) - 1) / chunk_columns(dtype); }
+// of the sorted entries, none where they are few
+size_t sorted_bytes(int64_t n_rows, int64_t vocab, int dtype, int k) {
+  if (k <= kUnsortedEntries) return 0;
+  return 2 * align_up((size_t)n_rows * k * 4, 256) + align_up((size_t)n_rows * (chunks_of(vocab, dtype) + 1) * 4, 256);
+}
+Sorted carve_sorted(void* buffer, int64_t n_rows, int64_t vocab, int dtype, int k) {
+  Sorted to{};
+  if (k <= kUnsortedEntries || !buffer) return to;
+  to.chunks = (int)chunks_of(vocab, dtype);
+  to.chunk_cols = chunk_columns(dtype);
+  Carver carve(buffer);
+  to.column = carve.take<int>((size_t)n_rows * k);
+  to.grad = carve.take<float>((size_t)n_rows * k);
+  to.first = carve.take<int>((size_t)n_rows * (to.chunks + 1));
+  return to;
+}
+size_t entries_bytes(int64_t n_rows, int64_t vocab, int dtype, int k) {
+  const size_t many = sorted_bytes(n_rows, vocab, dtype, k);
+  return many ? many : (size_t)n_rows * k * 4;
 }
 int check_backward(const char* what, const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t ld, int k,
                    float rcp_temperature, const float* stats, const void* d_logits, int64_t ld_out) {
@@ -886,21 +977,21 @@ int check_backward(const char* what, const void* logits, int dtype, int64_t n_ro
   if (st != VAMD_OK) return st;
   VAMD_REQUIRE(stats && reinterpret_cast<uintptr_t>(stats) % 16 == 0, "%s: stats must be given, 16-byte aligned", what);
   VAMD_REQUIRE(d_logits && ld_out >= vocab && d_logits != logits, "%s: bad output", what);
-  VAMD_DTYPE_DISPATCH(dtype, D, {
-    VAMD_REQUIRE(n_rows * backward_chunks<D>(vocab) < (1ll << 31), "%s: too many workgroups", what);
-  });
+  VAMD_REQUIRE(n_rows * chunks_of(vocab, dtype) < (1ll << 31), "%s: too many workgroups", what);
   return VAMD_OK;
 }
 int entries_backward(EntriesArgs a, int dtype, int64_t n_rows, hipStream_t s) {
+  a.chunks = (int)chunks_of(a.cols, dtype);
+  const bool sorted = a.sorted.column != nullptr;
   VAMD_DTYPE_DISPATCH(dtype, D, {
-    const int64_t chunks = backward_chunks<D>(a.cols);
-    a.chunks = (int)chunks;
     const bool vec = rows_vectorizable<D>(a.logits, a.ld) && rows_vectorizable<D>(a.out, a.ld_out);
     const bool stream = cached_rows(n_rows, a.ld, sizeof(typename D::type)) < n_rows;
-    void (*const kernels[2][2])(EntriesArgs) = {
-        {row_entries_backward_kernel<D, false, false>, row_entries_backward_kernel<D, false, true>},
-        {row_entries_backward_kernel<D, true, false>, row_entries_backward_kernel<D, true, true>}};
-    hipLaunchKernelGGL(kernels[vec][stream], dim3((unsigned)(n_rows * chunks)), dim3(kNarrow), 0, s, a);
+    void (*const kernels[2][2][2])(EntriesArgs) = {
+        {{row_entries_backward_kernel<D, false, false, false>, row_entries_backward_kernel<D, false, false, true>},
+         {row_entries_backward_kernel<D, false, true, false>, row_entries_backward_kernel<D, false, true, true>}},
+        {{row_entries_backward_kernel<D, true, false, false>, row_entries_backward_kernel<D, true, false, true>},
+         {row_entries_backward_kernel<D, true, true, false>, row_entries_backward_kernel<D, true, true, true>}}};
+    hipLaunchKernelGGL(kernels[vec][stream][sorted], dim3((unsigned)(n_rows * a.chunks)), dim3(kNarrow), 0, s, a);
   });
   VAMD_LAUNCH_CHECK();
   return VAMD_OK;
@@ -970,35 +1061,61 @@ extern "C" int vamd_row_topk(const void* logits, int dtype, int64_t n_rows, int6
   return VAMD_OK;
 }
 
+extern "C" size_t vamd_row_topk_backward_workspace_bytes(int64_t n_rows, int64_t vocab, int dtype, int k) {
+  if (n_rows <= 0 || vocab <= 0 || k <= 0 || k > kMaxK) return 0;
+  return align_up((size_t)n_rows * 4, 256) + sorted_bytes(n_rows, vocab, dtype, k);
+}
+
 extern "C" int vamd_row_topk_backward(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t ld,
                                       const int64_t* labels, int k, const int64_t* index, float rcp_temperature,
                                       const float* stats, const float* d_logprobs, const float* d_entropy,
-                                      const float* d_top, float* row_scratch, void* d_logits, int64_t ld_out, void* stream) {
+                                      const float* d_top, void* d_logits, int64_t ld_out, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
   const int st = check_backward("row_topk_backward", logits, dtype, n_rows, vocab, ld, k, rcp_temperature, stats, d_logits, ld_out);
   if (st != VAMD_OK) return st;
-  VAMD_REQUIRE(row_scratch, "row_topk_backward: null pointer");
   VAMD_REQUIRE(d_logprobs || d_entropy || d_top, "row_topk_backward: no upstream gradient");
   VAMD_REQUIRE((!d_logprobs || labels) && (!d_top || index), "row_topk_backward: gradients of log-probs need their tokens");
+  const size_t need = vamd_row_topk_backward_workspace_bytes(n_rows, vocab, dtype, k);
+  if (!workspace || workspace_bytes < need) {
+    set_error("row_topk_backward: workspace %zu bytes, need %zu", workspace_bytes, need);
+    return VAMD_EWORKSPACE;
+  }
   hipStream_t s = static_cast<hipStream_t>(stream);
+  float* const weight = static_cast<float*>(workspace);
   const int entries = d_top ? k : 0;
-  hipLaunchKernelGGL(row_topk_weight_kernel, dim3((unsigned)((n_rows + kNarrow / 64 - 1) / (kNarrow / 64))), dim3(kNarrow), 0,
-                     s, d_logprobs, labels, vocab, d_top, entries, n_rows, row_scratch);
+  const Sorted sorted =
+      carve_sorted(static_cast<char*>(workspace) + align_up((size_t)n_rows * 4, 256), n_rows, vocab, dtype, entries);
+  hipLaunchKernelGGL(row_topk_prepare_kernel, dim3((unsigned)n_rows), dim3(kNarrow), 0, s, d_logprobs, labels, vocab, d_top, index,
+                     entries, weight, sorted);
   VAMD_LAUNCH_CHECK();
-  EntriesArgs a{logits, ld, vocab, 0, entries, index, d_top, reinterpret_cast<const float4*>(stats), row_scratch, nullptr,
-                labels, d_logprobs, d_entropy, rcp_temperature * kLog2e, rcp_temperature, d_logits, ld_out};
-  return entries_backward(a, dtype, n_rows, s);
+  return entries_backward(EntriesArgs{logits, ld, vocab, 0, entries, index, d_top, sorted, reinterpret_cast<const float4*>(stats),
+                                      weight, nullptr, labels, d_logprobs, d_entropy, rcp_temperature * kLog2e, rcp_temperature,
+                                      d_logits, ld_out},
+                          dtype, n_rows, s);
+}
+
+extern "C" size_t vamd_row_divergence_entries_bytes(int64_t n_rows, int64_t vocab, int dtype, int k) {
+  if (n_rows <= 0 || vocab <= 0 || k <= 0 || k > kMaxK) return 0;
+  return entries_bytes(n_rows, vocab, dtype, k);
 }
 
 extern "C" int vamd_row_divergence(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t ld,
                                    const float* teacher_logprobs, const int64_t* teacher_index, int k, int divergence,
-                                   float beta, float rcp_temperature, float* loss, float* stats, float* slope, void* stream) {
+                                   float beta, float rcp_temperature, float* loss, float* stats, void* entries,
+                                   size_t entries_size, void* stream) {
   int st = check_topk("row_divergence", logits, dtype, n_rows, vocab, ld, k, rcp_temperature);
   if (st != VAMD_OK) return st;
   if ((st = check_divergence("row_divergence", k, divergence, beta)) != VAMD_OK) return st;
   VAMD_REQUIRE(teacher_logprobs && teacher_index && loss, "row_divergence: null pointer");
   VAMD_REQUIRE(reinterpret_cast<uintptr_t>(stats) % 16 == 0, "row_divergence: stats must be 16-byte aligned");
+  VAMD_REQUIRE((stats == nullptr) == (entries == nullptr), "row_divergence: stats and entries are written together or not at all");
+  if (entries && entries_size < entries_bytes(n_rows, vocab, dtype, k)) {
+    set_error("row_divergence: entries of %zu bytes, need %zu", entries_size, entries_bytes(n_rows, vocab, dtype, k));
+    return VAMD_EWORKSPACE;
+  }
   DivergenceArgs a{logits, ld, vocab, teacher_logprobs, teacher_index, k, divergence, beta, rcp_temperature * kLog2e, loss,
-                   reinterpret_cast<float4*>(stats), slope, 0};
+                   reinterpret_cast<float4*>(stats), k <= kUnsortedEntries ? static_cast<float*>(entries) : nullptr,
+                   carve_sorted(entries, n_rows, vocab, dtype, k), 0};
   hipStream_t s = static_cast<hipStream_t>(stream);
   VAMD_DTYPE_DISPATCH(dtype, D, {
     a.cached_rows = cached_rows(n_rows, ld, sizeof(typename D::type));
@@ -1011,13 +1128,15 @@ extern "C" int vamd_row_divergence(const void* logits, int dtype, int64_t n_rows
 
 extern "C" int vamd_row_divergence_backward(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t ld,
                                             const int64_t* teacher_index, int k, float rcp_temperature, const float* stats,
-                                            const float* slope, const float* d_loss, void* d_logits, int64_t ld_out,
+                                            const void* entries, const float* d_loss, void* d_logits, int64_t ld_out,
                                             void* stream) {
   const int st = check_backward("row_divergence_backward", logits, dtype, n_rows, vocab, ld, k, rcp_temperature, stats, d_logits,
                                 ld_out);
   if (st != VAMD_OK) return st;
-  VAMD_REQUIRE(teacher_index && slope && d_loss, "row_divergence_backward: null pointer");
-  EntriesArgs a{logits, ld, vocab, 0, k, teacher_index, slope, reinterpret_cast<const float4*>(stats), nullptr, d_loss,
-                nullptr, nullptr, nullptr, rcp_temperature * kLog2e, rcp_temperature, d_logits, ld_out};
-  return entries_backward(a, dtype, n_rows, static_cast<hipStream_t>(stream));
+  VAMD_REQUIRE(teacher_index && entries && d_loss, "row_divergence_backward: null pointer");
+  return entries_backward(EntriesArgs{logits, ld, vocab, 0, k, teacher_index, static_cast<const float*>(entries),
+                                      carve_sorted(const_cast<void*>(entries), n_rows, vocab, dtype, k),
+                                      reinterpret_cast<const float4*>(stats), nullptr, d_loss, nullptr, nullptr, nullptr,
+                                      rcp_temperature * kLog2e, rcp_temperature, d_logits, ld_out},
+                          dtype, n_rows, static_cast<hipStream_t>(stream));
 }

@@ -592,13 +592,15 @@ class RowTopk : public torch::autograd::Function<RowTopk> {
                    g_lp = grads.size() > 3 ? upstream_rows(grads[3], dev) : Tensor();
       if (g_ent.defined() || g_top.defined() || g_lp.defined()) {
         const Tensor lab = saved[1].defined() ? saved[1].contiguous() : Tensor(), index = saved[2].contiguous(),
-                     stats = saved[3].contiguous(), scratch = new_f32({r.n()}, dev);
+                     stats = saved[3].contiguous();
+        const int64_t bytes = (int64_t)vamd_row_topk_backward_workspace_bytes(r.n(), r.vocab(), r.type, (int)index.size(-1));
+        const Tensor ws = at::empty({bytes}, index.options().dtype(at::kByte));
         d = at::empty(shape, r.t.options());
         check(vamd_row_topk_backward(r.data(), r.type, r.n(), r.vocab(), r.ld,
                                      lab.defined() ? lab.const_data_ptr<int64_t>() : nullptr, (int)index.size(-1),
                                      index.const_data_ptr<int64_t>(), (float)ctx->saved_data["rcp"].toDouble(), f32(stats),
-                                     f32(g_lp), f32(g_ent), f32(g_top), f32_out(scratch), d.mutable_data_ptr(), r.vocab(),
-                                     stream_of(dev)));
+                                     f32(g_lp), f32(g_ent), f32(g_top), d.mutable_data_ptr(), r.vocab(), ws.mutable_data_ptr(),
+                                     bytes, stream_of(dev)));
       }
     }
     return {once_differentiable(d, records, grads), Tensor(), Tensor(), Tensor()};
@@ -648,17 +650,19 @@ Teacher teacher_rows(const Tensor& logprobs, const Tensor& index, at::IntArrayRe
 }
 
 struct DivergenceResult {
-  Tensor loss, stats, slope;
+  Tensor loss, stats, entries;
 };
 DivergenceResult row_divergence(const Tensor& logits, const Rows& r, const Teacher& t, int kind, float beta, float rcp,
                                 bool need_grad) {
   const at::Device dev = logits.device();
   const c10::DeviceGuard guard(dev);
+  const int64_t bytes = need_grad ? (int64_t)vamd_row_divergence_entries_bytes(r.n(), r.vocab(), r.type, t.k()) : 0;
   const DivergenceResult out{
       at::empty(logits.sizes().slice(0, logits.dim() - 1), at::TensorOptions().dtype(at::kFloat).device(dev)),
-      need_grad ? new_f32({r.n(), 4}, dev) : Tensor(), need_grad ? new_f32({r.n(), t.k()}, dev) : Tensor()};
+      need_grad ? new_f32({r.n(), 4}, dev) : Tensor(), need_grad ? at::empty({bytes}, t.index.options().dtype(at::kByte)) : Tensor()};
   check(vamd_row_divergence(r.data(), r.type, r.n(), r.vocab(), r.ld, f32(t.logprobs), t.index.const_data_ptr<int64_t>(), t.k(),
-                            kind, beta, rcp, f32_out(out.loss), f32_out(out.stats), f32_out(out.slope), stream_of(dev)));
+                            kind, beta, rcp, f32_out(out.loss), f32_out(out.stats),
+                            need_grad ? out.entries.mutable_data_ptr() : nullptr, bytes, stream_of(dev)));
   return out;
 }
 
@@ -669,7 +673,7 @@ class RowDivergence : public torch::autograd::Function<RowDivergence> {
     const Rows r = logit_rows(logits);
     const Teacher t = teacher_rows(logprobs, index, logits.sizes().slice(0, logits.dim() - 1), logits.device());
     const DivergenceResult out = row_divergence(logits, r, t, (int)kind, (float)beta, (float)rcp, true);
-    ctx->save_for_backward({r.t, t.index, out.stats, out.slope});
+    ctx->save_for_backward({r.t, t.index, out.stats, out.entries});
     ctx->saved_data["logits_shape"] = logits.sizes().vec();
     ctx->saved_data["rcp"] = rcp;
     return out.loss;
@@ -685,11 +689,11 @@ class RowDivergence : public torch::autograd::Function<RowDivergence> {
       const at::Device dev = r.t.device();
       const c10::DeviceGuard guard(dev);
       const Tensor g = upstream_rows(grads[0], dev), index = saved[1].contiguous(), stats = saved[2].contiguous(),
-                   slope = saved[3].contiguous();
+                   entries = saved[3].contiguous();
       d = at::empty(shape, r.t.options());
       check(vamd_row_divergence_backward(r.data(), r.type, r.n(), r.vocab(), r.ld, index.const_data_ptr<int64_t>(),
-                                         (int)index.size(-1), (float)ctx->saved_data["rcp"].toDouble(), f32(stats), f32(slope),
-                                         f32(g), d.mutable_data_ptr(), r.vocab(), stream_of(dev)));
+                                         (int)index.size(-1), (float)ctx->saved_data["rcp"].toDouble(), f32(stats),
+                                         entries.const_data_ptr(), f32(g), d.mutable_data_ptr(), r.vocab(), stream_of(dev)));
     }
     return {once_differentiable(d, records, grads), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
