@@ -137,6 +137,22 @@ def test_topk_of_views_and_without_labels(dev):
             assert (a - b).abs().max().item() <= 2 * _sum_error(3001) + 24 * U * 20
 
 
+@gpu
+def test_one_row_without_dimensions(dev):
+    """A vector of logits is one row: the label and the scalars have no dimension, the alternatives one."""
+    import verl_amd.utils.torch_functional as F
+    z = _logits((5001,), torch.float32, 8).to(dev).requires_grad_()
+    lp, ent, top, index = F.topk_logprobs_from_logits(z, torch.tensor(7, device=dev), 3)
+    rows = F.topk_logprobs_from_logits(z.detach()[None], torch.tensor([7], device=dev), 3)
+    assert lp.shape == ent.shape == () and top.shape == index.shape == (3,)
+    for a, b in zip((lp, ent, top, index), rows):
+        assert torch.equal(a, b[0])
+    loss = F.topk_distillation_from_logits(z, top.detach(), index)
+    assert loss.shape == () and abs(loss.item()) <= 8 * U * 30
+    d, = torch.autograd.grad((lp, loss), z)
+    assert d.shape == z.shape
+
+
 def _gradient_bound(want, q, weight, dtype, v, reach):
     e = _sum_error(v) + 8 * U * reach
     return HALF_STEP[dtype] * want.abs() * 1.01 + 2 * e * (q * weight.abs() + want.abs()) + torch.finfo(dtype).tiny * 2.0 ** -9
@@ -387,9 +403,16 @@ def test_capture_beside_an_eager_graph_of_the_same_leaf_is_refused(dev):
                 fn()
         torch.cuda.synchronize()
         del alive
-        with torch.cuda.graph(torch.cuda.CUDAGraph()):
-            fn()
-        torch.cuda.synchronize()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            elsewhere = fn()   # on a stream that can join a capture
+        torch.cuda.current_stream().wait_stream(side)
+        for kept in (elsewhere, None):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                fn()
+            torch.cuda.synchronize()
+            elsewhere = kept = None
 
 
 @gpu

@@ -180,6 +180,34 @@ def test_distillation_of_padded_and_repeated_entries(dev, monkeypatch, cache):
 
 
 @gpu
+def test_token_tiles_shared_out_in_bands_and_in_splits(dev):
+    """24 token tiles x 200 vocabulary tiles run in bands, a sixth of the tokens in splits: the same alternatives and losses."""
+    from verl_amd import _cabi
+    from verl_amd.utils.kernel.linear_topk import linear_topk_distillation, linear_topk_logprobs
+    n, h, v, k = 6144, 128, 51200, 12
+    hidden, weight = (x.to(dev) for x in _head(n, h, v, 3))
+    labels = torch.randint(0, v, (n,), device=dev)
+    e = 2 * _error(hidden[:64].cpu(), weight[:2000].cpu(), 1.0) * 1.5   # (the largest of a part of the sums; the rest by a half)
+    whole = linear_topk_logprobs(hidden, weight, labels, k)
+    parts = [linear_topk_logprobs(hidden[i:i + 1024], weight, labels[i:i + 1024], k) for i in range(0, n, 1024)]
+    L = _cabi.lib()
+    # the partial states tell which way the tiles are shared out: 10 splits of 24 tiles, or (3 bands + 8 XCDs) x 32 columns
+    assert L.vamd_lce_forward_workspace_bytes(n, h, v) == 11 * 32 * 256 * 20
+    for i, name in enumerate(("logprobs", "entropy", "top", "index")):
+        part = torch.cat([p[i] for p in parts])
+        if name == "index":
+            assert torch.equal(whole[i], part)
+        else:
+            assert (whole[i] - part).abs().max().item() <= e * 15, name
+    hd = hidden.clone().requires_grad_()
+    loss = linear_topk_distillation(hd, weight, whole[2] - 0.2, whole[3], "jsd")
+    part = torch.cat([linear_topk_distillation(hidden[i:i + 1024], weight, whole[2][i:i + 1024] - 0.2, whole[3][i:i + 1024], "jsd")
+                      for i in range(0, n, 1024)])
+    assert (loss - part).abs().max().item() <= 4 * e
+    assert torch.isfinite(torch.autograd.grad(loss.sum(), hd)[0]).all()
+
+
+@gpu
 @pytest.mark.parametrize("need", [(True, False), (False, True)])
 def test_distillation_with_one_frozen_input(dev, need):
     hidden, weight = _head(300, 256, 2000, 8)
@@ -296,7 +324,7 @@ def test_refusals(dev):
     for k in (0, 257, 301, 2.0):
         with pytest.raises(AssertionError, match="k must be"):
             linear_topk_logprobs(hidden, weight, labels, k)
-    for temperature in (0.0, -1.0, INF, NAN, 1):
+    for temperature in (0.0, -1.0, INF, NAN, 1, 1e-320):
         with pytest.raises(AssertionError, match="temperature"):
             linear_topk_logprobs(hidden, weight, labels, 2, temperature)
     for bad in ((hidden.float(), weight, labels), (hidden, weight[:, :64], labels), (hidden, weight.t().contiguous().t(), labels),
@@ -344,7 +372,7 @@ def test_refusals_on_the_host():
     topk = lambda hidden=at, n=4, h=128, v=300, k=5, rcp=1.0, labels=at, top=at, ws=at, size=1 << 40: lib.vamd_lce_topk(
         hidden, at, labels, n, h, v, k, rcp, at, at, top, at, 0, ws, size, None)
     for bad in (dict(hidden=None), dict(n=0), dict(h=100), dict(v=0), dict(k=0), dict(k=257), dict(k=301), dict(rcp=0.0),
-                dict(rcp=NAN), dict(labels=None), dict(top=None)):
+                dict(rcp=NAN), dict(rcp=INF), dict(labels=None), dict(top=None)):
         assert topk(**bad) == -1, bad
     need = lib.vamd_lce_topk_workspace_bytes(4, 128, 300, 5, 0)
     assert topk(size=need - 1) == -2 and topk(ws=None) == -2
@@ -352,7 +380,7 @@ def test_refusals_on_the_host():
     div = lambda hidden=at, cache=None, v=300, teacher=at, k=5, kind=0, beta=0.5, rcp=1.0, slope=at, prob=at: lib.vamd_lce_divergence(
         hidden, at, cache, 4, 128, v, teacher, at, k, kind, beta, rcp, at, at, at, at, slope, prob, None)
     for bad in (dict(hidden=None), dict(hidden=at + 8), dict(cache=at, v=300 + 1), dict(teacher=None), dict(k=0), dict(k=257),
-                dict(kind=3), dict(kind=2, beta=0.0), dict(rcp=-1.0), dict(slope=None), dict(prob=None)):
+                dict(kind=3), dict(kind=2, beta=0.0), dict(rcp=-1.0), dict(rcp=INF), dict(slope=None), dict(prob=None)):
         assert div(**bad) == -1, bad
     back = lambda index=at, k=5, d_loss=at, d_hidden=at, rcp=1.0, size=1 << 40: lib.vamd_lce_divergence_backward(
         at, at, at, 4, 4, 128, 300, index, k, rcp, at, at, at, at, d_loss, at, None, None, d_hidden, at, _cabi.DW_STORE, None, 0,

@@ -2297,6 +2297,7 @@ extern "C" int vamd_lce_divergence_forward(const void* hidden, const void* weigh
                               mean_z, logits_cache);
   if (st != VAMD_OK) return st;
   VAMD_REQUIRE(lse_rest, "lce_divergence_forward: null pointer");
+  VAMD_REQUIRE(rcp_temperature < __builtin_huge_valf(), "lce_divergence_forward: temperature must be positive");
   const size_t need = vamd_lce_forward_workspace_bytes(n_tokens, hidden_size, vocab);
   if (!workspace || workspace_bytes < need) {
     set_error("lce_divergence_forward: workspace %zu bytes, need %zu", workspace_bytes, need);
@@ -2320,7 +2321,7 @@ extern "C" int vamd_lce_divergence(const void* hidden, const void* weight, const
                "lce_divergence: slope_sum, slope and prob are written together or not at all");
   VAMD_REQUIRE((reinterpret_cast<uintptr_t>(hidden) | reinterpret_cast<uintptr_t>(weight)) % 16 == 0,
                "lce_divergence: hidden and weight must be 16-byte aligned");
-  VAMD_REQUIRE(rcp_temperature > 0.f, "lce_divergence: temperature must be positive");
+  VAMD_REQUIRE(rcp_temperature > 0.f && rcp_temperature < __builtin_huge_valf(), "lce_divergence: temperature must be positive");
   const HeadDivergenceArgs a{static_cast<const uint16_t*>(hidden), static_cast<const uint16_t*>(weight), logits_cache, lse,
                              lse_rest, teacher_logprobs, teacher_index, vocab, (int)n_tokens, (int)hidden_size, k, divergence, beta,
                              rcp_temperature, loss, slope_sum, slope, prob};
@@ -2392,7 +2393,7 @@ extern "C" int vamd_lce_topk(const void* hidden, const void* weight, const int64
   if (st != VAMD_OK) return st;
   VAMD_REQUIRE(hidden && weight && labels && logprobs && entropy && top && index, "lce_topk: null pointer");
   VAMD_REQUIRE(k >= 1 && k <= VAMD_TOPK_MAX && k <= vocab, "lce_topk: k is %d, of 1 to %d and the vocabulary", k, VAMD_TOPK_MAX);
-  VAMD_REQUIRE(rcp_temperature > 0.f, "lce_topk: temperature must be positive");
+  VAMD_REQUIRE(rcp_temperature > 0.f && rcp_temperature < __builtin_huge_valf(), "lce_topk: temperature must be positive");
   const size_t need = vamd_lce_topk_workspace_bytes(n_tokens, hidden_size, vocab, k, token_chunk);
   if (!workspace || workspace_bytes < need) {
     set_error("lce_topk: workspace %zu bytes, need %zu", workspace_bytes, need);

@@ -500,8 +500,8 @@ Tensor entropy_from_logits(const Tensor& logits, bool fp32_output) {
 
 // ---- top alternatives of materialised logits, and their divergence from a teacher's -----------------------------
 // At the end of a backward pass autograd makes the caller's stream wait for those of the leaves' accumulators.  One that an eager
-// graph of the same leaf keeps alive belongs to that graph's stream: under capture the wait records an event of a stream that is
-// not captured, and ending the capture ends the process.
+// graph of the same leaf keeps alive belongs to that graph's stream.  Under capture that stream joins the capture, unless it is the
+// default one, which cannot: then ending the capture ends the process.
 void refuse_capture_beside_eager_graph(const char* what, const Tensor& input) {
   if (!input.defined() || !input.is_cuda() || !input.is_leaf() || !input.requires_grad()) return;
   const c10::DeviceGuard guard(input.device());
@@ -509,9 +509,9 @@ void refuse_capture_beside_eager_graph(const char* what, const Tensor& input) {
   const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(input);
   if (!accumulator) return;
   const auto stream = accumulator->stream();
-  const auto mine = c10::hip::getCurrentHIPStream(input.device().index());
-  TORCH_CHECK(!stream || stream->id() == mine.id(), what, " cannot be captured while an eager graph of the same leaf is alive: "
-              "delete what was computed from it outside the capture");
+  const auto outside = c10::hip::getDefaultHIPStream(input.device().index());
+  TORCH_CHECK(!stream || stream->id() != outside.id(), what, " cannot be captured while an eager graph of the same leaf on the "
+              "default stream is alive: delete what was computed from it outside the capture");
 }
 void refuse_trace(const char* what) {
   TORCH_CHECK(!torch::jit::tracer::isTracing(), what, " cannot be recorded by torch.jit.trace");
