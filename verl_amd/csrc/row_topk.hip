@@ -770,8 +770,11 @@ struct EntriesArgs {
 // in order, in the registers of the lane that holds its column, so that an index that comes twice counts twice and each gradient
 // is rounded once.  Up to 64 entries every wavefront looks through all of the row's for its own: they come with the logits.  More
 // are sorted first, and a workgroup reads its own, behind the place of the first.  4096 x 152064 bf16, forward and backward pass of the
-// divergence, all of them looked through and sorted, us: 5 entries 606 and 605, 64 618 and 632, 128 690 and 649, 256 850 and 683.
-template <class D, bool VEC, bool STREAM, bool SORTED>
+// divergence, us: 64 entries 581, 65 (sorted) 592, 128 607, 256 636; with every wavefront looking through all of them, before the
+// arithmetic below was trimmed, 5 entries 606, 64 618, 128 690, 256 850.
+// ENTROPY: an entropy has an upstream gradient.  Bound by HBM (6.4 TB/s).  With the label's comparison and the entropy's terms at every
+// element the vector ALU was 89 % busy, and the pass took 428 us with 64 entries, now 388.
+template <class D, bool VEC, bool STREAM, bool SORTED, bool ENTROPY>
 __global__ __launch_bounds__(kNarrow) void row_entries_backward_kernel(EntriesArgs a) {
   using T = typename D::type;
   constexpr int G = D::kVec, F = D::kBackwardLoads;
@@ -780,8 +783,8 @@ __global__ __launch_bounds__(kNarrow) void row_entries_backward_kernel(EntriesAr
   const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const T* __restrict__ row = static_cast<const T*>(a.logits) + r * a.ld;
   T* __restrict__ out = static_cast<T*>(a.out) + r * a.ld_out;
-  constexpr int64_t stride = (int64_t)kNarrow * G;
-  const int64_t first = (int64_t)chunk * stride * F, c0 = first + (int64_t)threadIdx.x * G;
+  constexpr int stride = kNarrow * G;
+  const int64_t first = (int64_t)chunk * stride * F, c0 = first + (int)threadIdx.x * G;
   u32x4_t raw[F];
 #pragma unroll
   for (int u = 0; u < F; ++u) {
@@ -807,10 +810,9 @@ __global__ __launch_bounds__(kNarrow) void row_entries_backward_kernel(EntriesAr
     __builtin_amdgcn_sched_barrier(0);
   }
   const float scale = (a.scale ? a.scale[r] : 1.f) * a.rcp_t;
-  const float glp = a.d_logprobs ? a.d_logprobs[r] * a.rcp_t : 0.f;
   const int64_t label = a.d_logprobs ? a.labels[r] : -1;
   const float u0 = scale * (a.weight ? a.weight[r] : st.z) * st.y;
-  const float u1 = a.d_entropy ? a.d_entropy[r] * a.rcp_t * a.rcp_t * st.y : 0.f;
+  const float u1 = ENTROPY ? a.d_entropy[r] * a.rcp_t * a.rcp_t * st.y : 0.f;
   float x[F][G];
 #pragma unroll
   for (int u = 0; u < F; ++u) {
@@ -822,35 +824,38 @@ __global__ __launch_bounds__(kNarrow) void row_entries_backward_kernel(EntriesAr
     } else {
       load_ragged<D>(row, c, a.cols, 0.f, x[u]);
     }
-    const int64_t hit64 = label - c;
-    const int hit = (hit64 >= 0 && hit64 < G) ? (int)hit64 : -1;
 #pragma unroll
     for (int e = 0; e < G; ++e) {
       const float z = x[u][e];
       const float ex = __builtin_amdgcn_exp2f(fmaf(z, a.scale2, -st.x));
-      const float t = fmaf(u1, fmaxf(z, -1.0e20f) - st.z, u0);  // below it q is 0, which -inf would make a NaN
-      x[u][e] = fmaf(-ex, a.d_entropy ? t : u0, hit == e ? glp : 0.f);
+      // a logit below -1e20 has a q of 0, which -inf would make a NaN
+      x[u][e] = -ex * (ENTROPY ? fmaf(u1, fmaxf(z, -1.0e20f) - st.z, u0) : u0);
     }
   }
+  // adds g to the column `at` of the chunk (what lies past the row is not stored)
+  const auto add = [&](int at, float g) {
+    const int mine = at / G % 64 == lane ? at / stride * G + at % G : -1;
+#pragma unroll
+    for (int u = 0; u < F; ++u)
+#pragma unroll
+      for (int e = 0; e < G; ++e) x[u][e] += mine == u * G + e ? g : 0.f;
+  };
+  const int64_t label_at = label - first;
+  if (label_at >= 0 && label_at < stride * F && (int)label_at / G % kNarrow / 64 == w) add((int)label_at, a.d_logprobs[r] * a.rcp_t);
   for (int e0 = e_begin; e0 < e_end; e0 += 64) {
     if (SORTED && e0 > e_begin && e0 + lane < e_end) {
       column = a.sorted.column[entries + e0 + lane];
       grad = a.sorted.grad[entries + e0 + lane];
     }
-    const int64_t rel64 = (int64_t)column - first;
-    const bool inside = e0 + lane < e_end && column < a.cols && rel64 >= 0 && rel64 < stride * F;
-    const int rel = inside ? (int)rel64 : 0;
-    uint64_t hits = __ballot(inside && rel / G % kNarrow / 64 == w);
+    const int64_t at64 = (int64_t)column - first;
+    const bool inside = e0 + lane < e_end && at64 >= 0 && at64 < stride * F;
+    const int at = inside ? (int)at64 : 0;
+    uint64_t hits = __ballot(inside && at / G % kNarrow / 64 == w);
     while (hits) {
       const int b = __ffsll((unsigned long long)hits) - 1;
       hits &= hits - 1;
-      const int at = __builtin_amdgcn_readlane(rel, b);
-      const float g = (SORTED ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(grad), b)) : a.grad[entries + b]) * scale;
-      const int mine = at / G % 64 == lane ? at / (int)stride * G + at % G : -1;
-#pragma unroll
-      for (int u = 0; u < F; ++u)
-#pragma unroll
-        for (int e = 0; e < G; ++e) x[u][e] += mine == u * G + e ? g : 0.f;
+      add(__builtin_amdgcn_readlane(at, b),
+          (SORTED ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(grad), b)) : a.grad[entries + b]) * scale);
     }
   }
 #pragma unroll
@@ -980,18 +985,23 @@ int check_backward(const char* what, const void* logits, int dtype, int64_t n_ro
   VAMD_REQUIRE(n_rows * chunks_of(vocab, dtype) < (1ll << 31), "%s: too many workgroups", what);
   return VAMD_OK;
 }
+template <class D, bool ENTROPY>
+void launch_backward(const EntriesArgs& a, bool vec, bool stream, bool sorted, int64_t n_rows, hipStream_t s) {
+  void (*const kernels[2][2][2])(EntriesArgs) = {
+      {{row_entries_backward_kernel<D, false, false, false, ENTROPY>, row_entries_backward_kernel<D, false, false, true, ENTROPY>},
+       {row_entries_backward_kernel<D, false, true, false, ENTROPY>, row_entries_backward_kernel<D, false, true, true, ENTROPY>}},
+      {{row_entries_backward_kernel<D, true, false, false, ENTROPY>, row_entries_backward_kernel<D, true, false, true, ENTROPY>},
+       {row_entries_backward_kernel<D, true, true, false, ENTROPY>, row_entries_backward_kernel<D, true, true, true, ENTROPY>}}};
+  hipLaunchKernelGGL(kernels[vec][stream][sorted], dim3((unsigned)(n_rows * a.chunks)), dim3(kNarrow), 0, s, a);
+}
 int entries_backward(EntriesArgs a, int dtype, int64_t n_rows, hipStream_t s) {
   a.chunks = (int)chunks_of(a.cols, dtype);
   const bool sorted = a.sorted.column != nullptr;
   VAMD_DTYPE_DISPATCH(dtype, D, {
     const bool vec = rows_vectorizable<D>(a.logits, a.ld) && rows_vectorizable<D>(a.out, a.ld_out);
     const bool stream = cached_rows(n_rows, a.ld, sizeof(typename D::type)) < n_rows;
-    void (*const kernels[2][2][2])(EntriesArgs) = {
-        {{row_entries_backward_kernel<D, false, false, false>, row_entries_backward_kernel<D, false, false, true>},
-         {row_entries_backward_kernel<D, false, true, false>, row_entries_backward_kernel<D, false, true, true>}},
-        {{row_entries_backward_kernel<D, true, false, false>, row_entries_backward_kernel<D, true, false, true>},
-         {row_entries_backward_kernel<D, true, true, false>, row_entries_backward_kernel<D, true, true, true>}}};
-    hipLaunchKernelGGL(kernels[vec][stream][sorted], dim3((unsigned)(n_rows * a.chunks)), dim3(kNarrow), 0, s, a);
+    const auto launch = a.d_entropy ? launch_backward<D, true> : launch_backward<D, false>;
+    launch(a, vec, stream, sorted, n_rows, s);
   });
   VAMD_LAUNCH_CHECK();
   return VAMD_OK;
