@@ -5,6 +5,8 @@
   ``entropy_from_logits_with_chunking`` (:224-263) -- as one online-softmax pass per row
   (``vamd_row_softmax_stats``) with an elementwise backward (``vamd_row_softmax_backward``), and ``clip_by_value``
   (:203-221);
+* ``topk_logprobs_from_logits`` and ``topk_distillation_from_logits``, which the reference has not: a teacher's top alternatives
+  and a student's loss on them, from materialised logits (through the head: ``utils/kernel/linear_topk.py``);
 * the masked reductions ``masked_sum`` / ``masked_mean`` / ``masked_var`` / ``masked_whiten`` (:266-339).
 
 Inputs of the masked reductions may live on the CPU (they are staged to the current GPU and the result is
