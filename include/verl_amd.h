@@ -249,7 +249,8 @@ int vamd_row_softmax_backward_add(const void* logits, int dtype, int64_t n_rows,
  *   top [n_rows, k] fp32 and index [n_rows, k]: the log-probs of the k largest logits, largest first, the lowest index first
  *   among equals (a NaN ranks below -inf), 1 <= k <= min(VAMD_TOPK_MAX, vocab);
  *   logprobs (needs labels; a label outside [0, vocab) yields 0) and entropy (a logit of -inf adds nothing): fp32 [n_rows], may
- *   be NULL; stats: fp32 [n_rows, 4], 16-byte aligned, for the backward pass, may be NULL.
+ *   be NULL; stats: fp32 [n_rows, 4], 16-byte aligned, for the backward pass, may be NULL.  A row masked throughout with the lowest
+ *   value of its type is uniform; one of -inf is NaN.
  * One pass over the logits.  Few rows are shared out over workgroups and need a workspace (0 bytes otherwise). */
 #define VAMD_TOPK_MAX 256
 size_t vamd_row_topk_workspace_bytes(int64_t n_rows, int64_t vocab, int dtype, int k);
@@ -257,7 +258,7 @@ int vamd_row_topk(const void* logits, int dtype, int64_t n_rows, int64_t vocab, 
                   float rcp_temperature, float* logprobs, float* entropy, float* top, int64_t* index, float* stats,
                   void* workspace, size_t workspace_bytes, void* stream);
 /* Its gradient for upstream gradients of logprobs, entropy [n_rows] and top [n_rows, k], fp32, each of which may be NULL.
- * d_logits has the element type of the logits, row pitch ld_out, and is another buffer. */
+ * d_logits has the element type of the logits, row pitch ld_out, and is another buffer.  A row whose upstream gradients are 0 gets 0. */
 size_t vamd_row_topk_backward_workspace_bytes(int64_t n_rows, int64_t vocab, int dtype, int k);
 int vamd_row_topk_backward(const void* logits, int dtype, int64_t n_rows, int64_t vocab, int64_t ld, const int64_t* labels,
                            int k, const int64_t* index, float rcp_temperature, const float* stats, const float* d_logprobs,

@@ -123,6 +123,51 @@ def test_topk_of_masked_logits(dev, dtype, n, k):
 
 
 @gpu
+@pytest.mark.parametrize("n", [1, 5, 600])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_masked_throughout(dev, dtype, n):
+    """A row of the type's lowest value is uniform over it, one of -inf is NaN; where a loss masks such rows out they get no gradient."""
+    import verl_amd.utils.torch_functional as F
+    v, k, low = 9001, 30, torch.finfo(dtype).min
+    z = _logits((n, v), dtype, 2)
+    z[0] = low
+    if n > 1:
+        z[1] = low
+        z[1, 5000:] = -INF   # 5000 logits of the lowest value, the others ruled out
+        z[2] = -INF
+        z[3, 4:] = low
+    labels = torch.full((n,), 3)
+    # The outputs hold 32 bits: low / 0.7 of the types with 8 exponent bits is -4.8e38, past fp32's -3.4e38, and so -inf there.
+    want = [x[:5] for x in O.topk_logprobs(z[:5].double(), labels[:5], k, 0.7)]
+    want[2] = want[2].float().double()
+    zd = z.to(dev).requires_grad_()
+    got = F.topk_logprobs_from_logits(zd, labels.to(dev), k, 0.7)
+    assert torch.equal(got[3][:5].cpu(), want[3])
+    # fp16's lowest value is a number like others to the walk: of row 0 the entropy is the difference of lse and mean(z) / T, which are
+    # 65504 / 0.7 = 9.4e4 both; each is off by a few of its roundings (U x 9.4e4 = 5.6e-3) and a mean by its sums' error: as above.
+    reach = (z[:5].double().nan_to_num(0, 0, 0).abs().amax(-1) / 0.7) * (dtype == torch.float16)
+    for a, b, name in zip(got[:3], want, ("logprobs", "entropy", "top")):
+        extra = (2 * _sum_error(v) + 24 * U) * reach if name == "entropy" else 0.0
+        _within(a[:5], b, 4 * (_sum_error(v) + 200 * U) + 12 * U * b.abs().nan_to_num(0, 0, 0) + extra, name)
+    t, index = _teacher(_logits((n, v), torch.float32, 3), 70, 4)
+    index[0, 0] = 8999
+    up = torch.zeros(n)
+    up[-1] = 1.0
+    loss = F.topk_distillation_from_logits(zd, t.to(dev), index.to(dev), "forward_kl", temperature=0.7)
+    uniform = (t[0].exp() * (t[0] + math.log(v))).sum()
+    assert abs(loss[0].item() - uniform.item()) <= 20 * (_sum_error(v) + 200 * U)
+    top, = torch.autograd.grad(got[2], zd, (up[:, None] * torch.ones(n, k)).to(dev), retain_graph=True)
+    both = torch.autograd.grad((got[0], got[1], loss), zd, (up.to(dev),) * 3)[0]
+    for d in (top, both):
+        assert torch.isfinite(d).all() and (n == 1 or not d[:-1].any())
+    if n == 1:   # of the uniform row: q = 1 / v
+        want_d = torch.full((v,), -float(k) / v / 0.7, dtype=torch.float64)
+        want_d[:k] += 1 / 0.7
+        _within(top[0], want_d, HALF_STEP[dtype] * 1.01 * want_d.abs() + 4 * _sum_error(v) * k / v + 8 * U * want_d.abs()
+                + torch.finfo(dtype).tiny * 2.0 ** -9, "gradient")
+
+
+@gpu
 def test_topk_of_views_and_without_labels(dev):
     """Rows off 16 bytes, a pitch wider than the vocabulary, a transposed tensor, leading dimensions."""
     import verl_amd.utils.torch_functional as F

@@ -27,14 +27,19 @@ constexpr float kInf = __builtin_huge_valf();
 struct Softmax {
   float m, s, sz;  // max y, sum 2^(y - m), sum 2^(y - m) z
 };
+// A row's state as its users have it: of z - shift, where shift is 0 but for rows of lowest().
+struct RowState : Softmax {
+  float shift;
+};
 __device__ __forceinline__ void merge(Softmax& a, const Softmax& b) {
   const float m = fmaxf(a.m, b.m);
   const float x = __builtin_amdgcn_exp2f(a.m - m), y = __builtin_amdgcn_exp2f(b.m - m);
   a = Softmax{m, a.s * x + b.s * y, a.sz * x + b.sz * y};
 }
 // log q of logit z; the lowest values of a type, which masks are made of, would overflow as y
-__device__ __forceinline__ float log_q(float z, float scale2, const Softmax& r) {
+__device__ __forceinline__ float log_q(float z, float scale2, const RowState& r) {
   const float log2_s = log2f(r.s);
+  z -= r.shift;
   return z < -1.0e30f ? fmaf(z, scale2 * kLn2, -(r.m + log2_s) * kLn2) : (fmaf(z, scale2, -r.m) - log2_s) * kLn2;
 }
 
@@ -72,8 +77,8 @@ __device__ __forceinline__ float add_trip(const float (&x)[kInFlight][G], float 
 }
 // The same sz where a logit is -inf, which adds 0 and not 0 x -inf, or NaN; read again, so that the trip's logits need not be held.
 template <class D>
-__device__ __forceinline__ float sum_with_masked(const typename D::type* row, int64_t c, int64_t stride, int64_t end,
-                                                           float scale2, float m) {
+__device__ __forceinline__ float sum_with_masked(const typename D::type* row, int64_t c, int64_t stride, int64_t end, float scale2,
+                                                 float m) {
   float sz = 0.f;
 #pragma unroll 1
   for (int u = 0; u < kInFlight; ++u, c += stride)
@@ -209,6 +214,48 @@ __device__ __forceinline__ void merge_wave(Softmax& st) {
   merge(b, in_lane(st, 48));
   merge(a, b);
   st = a;
+}
+
+// The state of a row without a logit that a walk can tell from -inf (s is 0: every y lies below kNegBig), taken from its largest
+// logit: a row masked throughout with the lowest value of its type is uniform, one of -inf is NaN.  Every thread of the workgroup
+// comes here.
+template <class D, int NT>
+__device__ __forceinline__ RowState lowest(const typename D::type* __restrict__ row, int64_t cols, float scale2) {
+  __shared__ float red[3][NT / 64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  float hi = -kInf, s = 0.f, sz = 0.f;
+#pragma unroll 1
+  for (int64_t c = threadIdx.x; c < cols; c += NT) hi = fmaxf(hi, to_float(row[c], D()));
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) hi = fmaxf(hi, __shfl_xor(hi, off, 64));
+  if (lane == 0) red[0][w] = hi;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < NT / 64; ++j) hi = fmaxf(hi, red[0][j]);
+#pragma unroll 1
+  for (int64_t c = threadIdx.x; c < cols; c += NT) {
+    const float z = to_float(row[c], D()) - hi;
+    const float ex = __builtin_amdgcn_exp2f(z * scale2);
+    s += ex;
+    sz = fmaf(ex, ex == 0.f ? 0.f : z, sz);
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    s += __shfl_xor(s, off, 64);
+    sz += __shfl_xor(sz, off, 64);
+  }
+  if (lane == 0) {
+    red[1][w] = s;
+    red[2][w] = sz;
+  }
+  __syncthreads();
+  s = sz = 0.f;
+#pragma unroll
+  for (int j = 0; j < NT / 64; ++j) {
+    s += red[1][j];
+    sz += red[2][j];
+  }
+  return RowState{{0.f, s, sz}, hi};
 }
 
 // ---- the k largest of a range of a row ------------------------------------------------------------------------
@@ -414,7 +461,7 @@ __device__ void pick_by_digits(PickLds<NT>& lds, uint64_t* list, const typename 
   rank_equal<D, NT>(lds, row, begin, end, order, need, kk - need, emit);
 }
 
-// Where the logits of a group lie that the walk has left a maximum of: kPieces() x 16 bytes.
+// Where the logits of a group lie that the walk has left a maximum of: pieces() x 16 bytes.
 template <class D, int NT>
 struct WalkLayout {
   using Word = GroupWord<D>;
@@ -505,7 +552,7 @@ struct TopkArgs {
   float* entropy;
   float* top;      // [rows][k]
   int64_t* index;  // [rows][k]
-  float4* stats;   // m, 1 / s, mean z, lse
+  float4* stats;   // m, 1 / s, mean of z - shift, shift
   int64_t cached_rows;
   int splits;  // of a row; more than one: each leaves its state and its k largest, for row_topk_join_kernel
   int64_t split_cols;
@@ -516,7 +563,7 @@ struct TopkArgs {
 struct RowResult {
   const TopkArgs& a;
   int64_t r;
-  Softmax st;
+  RowState st;
   __device__ __forceinline__ void operator()(int rank, uint64_t entry) const {
     a.top[r * a.k + rank] = log_q(logit_of(order_in(entry)), a.scale2, st);
     a.index[r * a.k + rank] = column_in(entry);
@@ -525,7 +572,7 @@ struct RowResult {
   __device__ __forceinline__ void scalars(const typename D::type* __restrict__ row) const {
     const float lse = (st.m + log2f(st.s)) * kLn2, mean = st.sz / st.s;
     if (a.entropy) a.entropy[r] = fmaf(-mean, a.rcp_t, lse);
-    if (a.stats) a.stats[r] = make_float4(st.m, 1.f / st.s, mean, lse);
+    if (a.stats) a.stats[r] = make_float4(st.m, 1.f / st.s, mean, st.shift);
     if (a.logprobs) {  // a label outside [0, cols) reads nothing and yields 0
       const int64_t label = a.labels[r];
       a.logprobs[r] = label >= 0 && label < a.cols ? log_q(to_float(row[label], D()), a.scale2, st) : 0.f;
@@ -558,7 +605,9 @@ __global__ __launch_bounds__(NT) void row_topk_kernel(TopkArgs a) {
     for (int64_t j = end - begin + threadIdx.x; j < a.k; j += NT) out[j] = 0;
     if (threadIdx.x == 0) a.part_state[part] = make_float4(st.m, st.s, st.sz, 0.f);
   } else {
-    const RowResult result{a, r, st};
+    RowState state{st, 0.f};
+    if (st.s == 0.f) state = lowest<D, NT>(row, a.cols, a.scale2);
+    const RowResult result{a, r, state};
     pick<D, VEC, NT>(lds, groups, layout, row, begin, end, a.k, best, result);
     if (threadIdx.x == 0) result.template scalars<D>(row);
   }
@@ -630,9 +679,12 @@ __global__ __launch_bounds__(kNarrow) void row_topk_join_kernel(TopkArgs a) {
     if (x >= least) list[atomicAdd(&found, 1)] = x;
   }
   __syncthreads();
-  const RowResult result{a, r, whole};
+  const auto* const row = static_cast<const typename D::type*>(a.logits) + r * a.ld;
+  RowState state{whole, 0.f};
+  if (whole.s == 0.f) state = lowest<D, kNarrow>(row, a.cols, a.scale2);
+  const RowResult result{a, r, state};
   rank_list<kNarrow>(list, found, a.k, result);
-  if (threadIdx.x == 0) result.template scalars<D>(static_cast<const typename D::type*>(a.logits) + r * a.ld);
+  if (threadIdx.x == 0) result.template scalars<D>(row);
 }
 
 // ---- divergence from a teacher's tokens -----------------------------------------------------------------------
@@ -682,7 +734,7 @@ struct DivergenceArgs {
   int k, kind;
   float beta, scale2;
   float* loss;
-  float4* stats;  // m, 1 / s, sum of the slopes, lse; null without a backward pass
+  float4* stats;  // m, 1 / s, sum of the slopes, shift; null without a backward pass
   float* slope;   // [rows][k], where the entries are few
   Sorted sorted;  // where they are many
   int64_t cached_rows;
@@ -717,8 +769,10 @@ __global__ __launch_bounds__(NT) void row_divergence_kernel(DivergenceArgs a) {
   st = Softmax{red[0][0], red[1][0], 0.f};
 #pragma unroll
   for (int j = 1; j < NT / 64; ++j) merge(st, Softmax{red[0][j], red[1][j], 0.f});
+  RowState state{st, 0.f};
+  if (st.s == 0.f) state = lowest<D, NT>(row, a.cols, a.scale2);
   Term mine{0.f, 0.f};
-  if (index >= 0) mine = divergence_term(a.kind, a.beta, t, log_q(z, a.scale2, st));
+  if (index >= 0) mine = divergence_term(a.kind, a.beta, t, log_q(z, a.scale2, state));
   if (a.slope && (int)threadIdx.x < a.k) a.slope[r * a.k + threadIdx.x] = mine.slope;
   if (a.sorted.column) sort_entries<NT>(a.sorted, r, a.k, index >= 0 ? (int)index : kNoEntry, mine.slope);
 #pragma unroll
@@ -741,7 +795,7 @@ __global__ __launch_bounds__(NT) void row_divergence_kernel(DivergenceArgs a) {
       slope += red[1][j];
     }
     a.loss[r] = loss;
-    if (a.stats) a.stats[r] = make_float4(st.m, 1.f / st.s, slope, (st.m + log2f(st.s)) * kLn2);
+    if (a.stats) a.stats[r] = make_float4(state.m, 1.f / state.s, slope, state.shift);
   }
 }
 static_assert(kMaxK <= kNarrow, "an entry per thread");
@@ -755,7 +809,7 @@ struct EntriesArgs {
   const int64_t* index;    // [rows][k]; one outside [0, cols) matches nothing
   const float* grad;       // [rows][k]: g_k
   Sorted sorted;           // the same where there are more than kUnsortedEntries
-  const float4* stats;     // m, 1 / s, ., .
+  const float4* stats;     // m, 1 / s, ., shift
   const float* weight;     // [rows]: sum of all g; null: the third of stats
   const float* scale;      // [rows] or null (1)
   const int64_t* labels;   // with d_logprobs
@@ -811,8 +865,10 @@ __global__ __launch_bounds__(kNarrow) void row_entries_backward_kernel(EntriesAr
   }
   const float scale = (a.scale ? a.scale[r] : 1.f) * a.rcp_t;
   const int64_t label = a.d_logprobs ? a.labels[r] : -1;
-  const float u0 = scale * (a.weight ? a.weight[r] : st.z) * st.y;
-  const float u1 = ENTROPY ? a.d_entropy[r] * a.rcp_t * a.rcp_t * st.y : 0.f;
+  const float g0 = scale * (a.weight ? a.weight[r] : st.z), g1 = ENTROPY ? a.d_entropy[r] * a.rcp_t * a.rcp_t : 0.f;
+  const float u0 = g0 * st.y, u1 = g1 * st.y;
+  // a row that no gradient comes to, such as one that a loss masks out: whatever its logits are
+  const bool none = g0 == 0.f && g1 == 0.f;
   float x[F][G];
 #pragma unroll
   for (int u = 0; u < F; ++u) {
@@ -823,6 +879,15 @@ __global__ __launch_bounds__(kNarrow) void row_entries_backward_kernel(EntriesAr
       for (int e = 0; e < G; ++e) x[u][e] = to_float(p.v[e], D());
     } else {
       load_ragged<D>(row, c, a.cols, 0.f, x[u]);
+    }
+    if (none) {
+#pragma unroll
+      for (int e = 0; e < G; ++e) x[u][e] = 0.f;
+      continue;
+    }
+    if (st.w != 0.f) {
+#pragma unroll
+      for (int e = 0; e < G; ++e) x[u][e] -= st.w;
     }
 #pragma unroll
     for (int e = 0; e < G; ++e) {
