@@ -269,6 +269,7 @@ int vamd_row_topk_backward(const void* logits, int dtype, int64_t n_rows, int64_
  *   VAMD_DIV_FORWARD_KL sum p (t - log q), VAMD_DIV_REVERSE_KL sum q (log q - t), VAMD_DIV_JSD beta sum p (t - log w) +
  *   (1 - beta) sum q (log q - log w) with w = beta p + (1 - beta) q, 0 < beta < 1.
  * An entry whose index lies outside [0, vocab) or whose t is -inf adds nothing; a row of such entries has loss 0 and no gradient.
+ * A row whose d_loss is 0 gets no gradient, also where its loss is NaN.
  * stats (fp32 [n_rows, 4], 16-byte aligned) and entries (vamd_row_divergence_entries_bytes() bytes, 256-byte aligned: what
  * d loss / d log q is at each entry) are what the backward pass needs, and are NULL together without one. */
 #define VAMD_DIV_FORWARD_KL 0

@@ -168,6 +168,25 @@ def test_rows_masked_throughout(dev, dtype, n):
 
 
 @gpu
+@pytest.mark.parametrize("kind", ["forward_kl", "reverse_kl", "jsd"])
+@pytest.mark.parametrize("k", [5, 100])
+def test_rows_out_of_the_loss_get_no_gradient(dev, kind, k):
+    """Rows of -inf and of NaN, whose divergence is NaN, beside rows that count: the upstream gradient decides."""
+    import verl_amd.utils.torch_functional as F
+    n, v = 6, 5003
+    z = _logits((n, v), torch.bfloat16, 2)
+    t, index = _teacher(_logits((n, v), torch.float32, 3), k, 4)
+    bad = z.clone()
+    bad[1], bad[4] = -INF, float("nan")
+    up = torch.tensor([0.5, 0.0, -1.0, 0.0, 0.0, 2.0]).to(dev)
+    grads = []
+    for x in (z, bad):
+        x = x.to(dev).requires_grad_()
+        grads.append(torch.autograd.grad(F.topk_distillation_from_logits(x, t.to(dev), index.to(dev), kind), x, up)[0])
+    assert torch.equal(*grads) and not grads[0][[1, 3, 4]].any() and grads[0][[0, 2, 5]].any()
+
+
+@gpu
 def test_topk_of_views_and_without_labels(dev):
     """Rows off 16 bytes, a pitch wider than the vocabulary, a transposed tensor, leading dimensions."""
     import verl_amd.utils.torch_functional as F

@@ -865,9 +865,12 @@ __global__ __launch_bounds__(kNarrow) void row_entries_backward_kernel(EntriesAr
   }
   const float scale = (a.scale ? a.scale[r] : 1.f) * a.rcp_t;
   const int64_t label = a.d_logprobs ? a.labels[r] : -1;
-  const float g0 = scale * (a.weight ? a.weight[r] : st.z), g1 = ENTROPY ? a.d_entropy[r] * a.rcp_t * a.rcp_t : 0.f;
+  // a token that a loss masks out, whose slopes may be NaN
+  const bool out_of_loss = a.scale && scale == 0.f;
+  if (out_of_loss) e_end = e_begin;
+  const float g0 = out_of_loss ? 0.f : scale * (a.weight ? a.weight[r] : st.z), g1 = ENTROPY ? a.d_entropy[r] * a.rcp_t * a.rcp_t : 0.f;
   const float u0 = g0 * st.y, u1 = g1 * st.y;
-  // a row that no gradient comes to, such as one that a loss masks out: whatever its logits are
+  // a row that no gradient comes to, whatever its logits are
   const bool none = g0 == 0.f && g1 == 0.f;
   float x[F][G];
 #pragma unroll
